@@ -69,13 +69,28 @@ class Config(ctypes.Structure):
         return f"Config({self.as_dict()})"
 
 
+class KVPages(ctypes.Structure):
+    """cq_kv_pages: the pages of a KV cache and how they lie in memory (see kv_pages, State.kv_pages)."""
+
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("k", "v", "k_scale", "v_scale")]
+                + [(f, ctypes.c_int64) for f in ("layer_stride", "page_stride", "head_stride")]
+                + [(f, ctypes.c_int32) for f in ("kv_dtype", "n_layers", "n_pages", "page_tokens", "n_kv_heads", "head_dim")])
+
+
+class PageMap(ctypes.Structure):
+    """cq_page_map: reference counts, tables and lengths of a pool's sequences (device pointers)."""
+
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("ref", "table", "len")]
+                + [(f, ctypes.c_int32) for f in ("n_pages", "n_seqs", "max_pages", "page_tokens")])
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
             f"{LIB_PATH} is not built; run `python cuqwen_amd/build.py` (or __graft_entry__.build())")
     lib = ctypes.CDLL(LIB_PATH)
     P, I32, U64, SZ, F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint64, ctypes.c_size_t, ctypes.c_float
-    CP = ctypes.POINTER(Config)
+    CP, GP, MP = ctypes.POINTER(Config), ctypes.POINTER(KVPages), ctypes.POINTER(PageMap)
     IP = ctypes.POINTER(ctypes.c_int32)
     sig = {
         "cq_last_error": (ctypes.c_char_p, []),
@@ -142,6 +157,19 @@ def _load():
         "cq_gqa_attention_decode_kv8": (I32, [P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, P, P]),
         "cq_gqa_attention_decode_fp8": (I32, [P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, P, P]),
         "cq_dequantize": (I32, [I32, I32, P, P, P, I32, I32, P]),
+        "cq_kv_pages_layout": (I32, [I32] * 6 + [GP, ctypes.POINTER(SZ), ctypes.POINTER(SZ)]),
+        "cq_state_kv_pages": (I32, [P, I32, GP]),
+        "cq_pages_fork": (I32, [MP, P, P, I32, P, P]),
+        "cq_pages_append": (I32, [GP, MP, P, P, I32, P, P, P]),
+        "cq_pages_workspace_bytes": (SZ, [MP]),
+        "cq_pages_trim": (I32, [MP, P, P, I32, P, P]),
+        "cq_pages_compact": (I32, [GP, MP, P, P, P, P]),
+        "cq_pages_copy": (I32, [GP, GP, P, P, I32, P, P]),
+        "cq_paged_kv_store": (I32, [GP, I32, P, P, ctypes.c_int64, P, I32, P]),
+        "cq_paged_kv_load": (I32, [GP, I32, P, P, ctypes.c_int64, P, I32, P]),
+        "cq_prefix_attention_decode": (I32, [P, ctypes.c_int64, P, ctypes.c_int64, GP, P, I32, P, GP, P, I32, P, P, I32, I32,
+                                             I32, P, P]),
+        "cq_prefix_attention_workspace_bytes": (SZ, [I32, I32, I32, I32]),
         "cq_time_gemv": (I32, [I32, I32, I32, ctypes.POINTER(P), ctypes.POINTER(P), P, P, I32, I32, I32,
                                ctypes.POINTER(ctypes.c_double)]),
         "cq_time_stream": (I32, [SZ, I32, ctypes.POINTER(P), I32, ctypes.POINTER(ctypes.c_double)]),
@@ -180,6 +208,9 @@ EXPORTED = [
     "cq_kv_cache_store", "cq_rope", "cq_gqa_attention_decode", "cq_attention_workspace_bytes", "cq_dequantize",
     "cq_kv_cache_store_hm", "cq_gqa_attention_decode_hm", "cq_gqa_attention_decode_noalloc",
     "cq_noalloc_scratch_bytes",
+    "cq_kv_pages_layout", "cq_state_kv_pages", "cq_pages_fork", "cq_pages_append", "cq_pages_workspace_bytes", "cq_pages_trim",
+    "cq_pages_compact", "cq_pages_copy", "cq_paged_kv_store", "cq_paged_kv_load", "cq_prefix_attention_decode",
+    "cq_prefix_attention_workspace_bytes",
     "cq_time_gemv", "cq_time_stream", "cq_time_grid_barrier", "cq_state_profile", "cq_tokenizer_load", "cq_tokenizer_free", "cq_tokenizer_encode",
     "cq_tokenizer_decode", "cq_tokenizer_token_id", "cq_tokenizer_vocab_size", "cq_chat_template",
 ]
@@ -294,6 +325,29 @@ def device_count():
     n = ctypes.c_int32(0)
     check(lib.cq_device_count(ctypes.byref(n)))
     return n.value
+
+
+# --------------------------------------------------------- paged KV cache
+def kv_pages(page_tokens, n_kv_heads, head_dim, n_pages, n_layers, kv_dtype=0, k=None, v=None, k_scale=None, v_scale=None):
+    """A pool's description (cq_kv_pages_layout) over device memory that the caller owns: k and v of
+    kv_pages_bytes()[0] bytes each, and for one-byte codes scales of [1]."""
+    p = KVPages()
+    check(lib.cq_kv_pages_layout(int(kv_dtype), n_layers, n_pages, page_tokens, n_kv_heads, head_dim, ctypes.byref(p), None, None))
+    p.k, p.v, p.k_scale, p.v_scale = k, v, k_scale, v_scale
+    return p
+
+
+def kv_pages_bytes(pages):
+    """(bytes of k, and of v; bytes of each scale array) of a pool as kv_pages lays it out."""
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+    check(lib.cq_kv_pages_layout(pages.kv_dtype, pages.n_layers, pages.n_pages, pages.page_tokens, pages.n_kv_heads,
+                                 pages.head_dim, ctypes.byref(KVPages()), ctypes.byref(a), ctypes.byref(b)))
+    return a.value, b.value
+
+
+def page_map(ref, table, length, n_pages, n_seqs, max_pages, page_tokens):
+    """cq_page_map over device memory that the caller owns: ref[n_pages], table[n_seqs][max_pages], length[n_seqs] (int32)."""
+    return PageMap(ref, table, length, n_pages, n_seqs, max_pages, page_tokens)
 
 
 # ------------------------------------------------------------ model level
@@ -411,6 +465,12 @@ class State:
     def kv_write(self, layer, kv_head, kind, arr):
         a = np.ascontiguousarray(arr, dtype=np.float16).view(np.uint16)
         check(lib.cq_state_kv_write(self.handle, layer, kv_head, kind, a.shape[0], a.ctypes.data))
+
+    def kv_pages(self, page_tokens):
+        """This state's cache as pages of page_tokens positions (cq_state_kv_pages); valid while the state lives."""
+        p = KVPages()
+        check(lib.cq_state_kv_pages(self.handle, page_tokens, ctypes.byref(p)))
+        return p
 
     def profile(self, pos, iters=3, max_kernels=16):
         names = ctypes.create_string_buffer(32 * max_kernels)

@@ -864,6 +864,20 @@ static size_t kv8_index(int kind, int t, int d, int ms, int hd) {
   return (size_t)(kind == 0 ? kv8_k_offset(0, t, d, ms, hd) : kv8_v_offset(0, t, d, ms, hd));
 }
 
+extern "C" int cq_state_kv_pages(cq_state* s, int32_t page_tokens, cq_kv_pages* out) {
+  if (!s || !out) return fail(CQ_EINVAL, "state_kv_pages: null argument");
+  const cq_config& c = s->cfg;
+  if (page_tokens < 1 || page_tokens > c.max_seq_len) return fail(CQ_EINVAL, "state_kv_pages: page_tokens outside [1, max_seq_len]");
+  // a head's positions follow each other in whole tiles: its pages lie one behind the other
+  CQ_TRY(cq_kv_pages_layout(s->kv_dtype, c.n_layers, c.max_seq_len / page_tokens, page_tokens, c.n_kv_heads, c.head_dim, out, nullptr, nullptr));
+  out->k = s->kcache; out->v = s->vcache;
+  out->k_scale = s->kscale; out->v_scale = s->vscale;
+  out->page_stride = (int64_t)page_tokens * c.head_dim;
+  out->head_stride = (int64_t)c.max_seq_len * c.head_dim;
+  out->layer_stride = (int64_t)s->layer_kv_halves;
+  return CQ_OK;
+}
+
 extern "C" int cq_state_kv_read(cq_state* s, int32_t layer, int32_t kv_head, int32_t kind, int32_t n_pos,
                                 uint16_t* host_out) {
   if (!s || !host_out) return fail(CQ_EINVAL, "kv_read: null argument");

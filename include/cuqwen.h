@@ -422,6 +422,152 @@ int cq_gqa_attention_decode_fp8(const void* q, const void* k_new, const void* v_
                                 int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_seq_len,
                                 void* workspace, void* stream);
 
+/* ------------------------------------------------------- paged KV cache */
+/* A KV cache of several sequences in pages, so that sequences which begin alike
+ * (the answers to one prompt) keep that beginning once.  No counterpart in the
+ * reference, whose cache holds one sequence (src/model.cu:37-38).
+ *
+ * A page holds the K and V of page_tokens consecutive positions of one sequence,
+ * for every kv head of every layer.  Within (layer, page, kv head) the elements
+ * are those of a layer cache of page_tokens slots: element (kv_head, t, d) of page
+ * p of layer l lies at l * layer_stride + p * page_stride + kv_head * head_stride +
+ * cq_kv_k_offset(0, t, d, page_tokens, head_dim) (V: cq_kv_v_offset; int8 / E4M3:
+ * cq_kv8_k_offset / cq_kv8_v_offset).  The fp32 scale of a one-byte row lies at the
+ * element offset of its (l, p, kv_head), divided by head_dim, plus t.
+ *
+ * page_tokens is a power of two in [32, 32768], n_pages at most 2^20, n_pages *
+ * page_tokens below 2^31.  k, v and the scales are aligned to 16 bytes.  The
+ * strides are multiples of 32 * head_dim; pages of one head follow each other (as
+ * in a state's own cache) or the heads of one page do. */
+typedef struct cq_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;          /* one-byte codes; else ignored */
+  float* v_scale;
+  int64_t layer_stride;    /* elements */
+  int64_t page_stride;
+  int64_t head_stride;
+  int32_t kv_dtype;        /* CQ_KV_* */
+  int32_t n_layers;
+  int32_t n_pages;
+  int32_t page_tokens;
+  int32_t n_kv_heads;
+  int32_t head_dim;        /* 64 or 128 */
+} cq_kv_pages;
+
+/* Fills in *out for a pool of its own, [n_layers][n_pages][n_kv_heads][page_tokens *
+ * head_dim], with null pointers; *kv_bytes receives the size of k (and of v),
+ * *scale_bytes that of each scale array (0 for fp16). */
+int cq_kv_pages_layout(int32_t kv_dtype, int32_t n_layers, int32_t n_pages, int32_t page_tokens, int32_t n_kv_heads,
+                       int32_t head_dim, cq_kv_pages* out, size_t* kv_bytes, size_t* scale_bytes);
+
+/* A state's own cache as pages: page p holds its positions [p * page_tokens, (p + 1) *
+ * page_tokens), so that a prompt that cq_prefill has put there can be read as a
+ * shared prefix, or copied into a pool.  n_pages = max_seq_len / page_tokens
+ * (rounded down).  Valid until the state is destroyed. */
+int cq_state_kv_pages(cq_state* s, int32_t page_tokens, cq_kv_pages* out);
+
+/* Which pages the sequences of a pool hold, in device memory.  Sequence s holds
+ * ceil(len[s] / page_tokens) pages, table[s * max_pages + i] its i-th one; ref[p]
+ * counts the tables that name page p (and what its user adds, to keep a page); a
+ * page with a count of zero or less is free.  Begin with ref and len zeroed.  At most 1024
+ * sequences, max_pages * page_tokens below 2^31. */
+typedef struct cq_page_map {
+  int32_t* ref;            /* [n_pages] */
+  int32_t* table;          /* [n_seqs][max_pages] */
+  int32_t* len;            /* [n_seqs], tokens */
+  int32_t n_pages;
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t page_tokens;
+} cq_page_map;
+
+/* The calls below are asynchronous on `stream`, allocate nothing and take their
+ * lists from device memory, so they can be captured; what they find wrong there
+ * they report in d_status (device memory, CQ_* codes) and leave alone.  Calls on
+ * one map or pool belong on one stream, or in an order of the caller's. */
+
+/* Each sequence d_child[i] (empty: len 0) becomes a copy of d_parent[i]: the same
+ * pages, counted once more; n is at most 1024.  d_status[i] (n ints): CQ_OK; CQ_ERANGE: an id outside
+ * [0, n_seqs), a parent whose len is out of range; CQ_EINVAL: the child is not empty,
+ * an earlier pair names it too, or the parent is a child of this call.  A refused pair
+ * changes nothing. */
+int cq_pages_fork(const cq_page_map* map, const int32_t* d_parent, const int32_t* d_child, int32_t n, int32_t* d_status,
+                  void* stream);
+
+/* Makes room for d_add[s] more tokens of every sequence s (n_seqs ints) and writes
+ * the slots of these tokens, sequence after sequence, to d_slots: slot = page *
+ * page_tokens + position % page_tokens, -1 in what is left of its n_slots ints.
+ * Where a sequence's first new token falls into a partly filled page that others
+ * hold too, the sequence gets a page of its own first, with the 32-token tiles that
+ * hold its tokens copied in every layer; of several that write to one page in the
+ * same call the last keeps it if nobody else holds it.  The pages that are taken
+ * are the free ones of lowest number, in the order of the sequences.
+ * d_status (4 ints): code, pages taken (or wanted), pages copied, tokens.  All or
+ * nothing: with CQ_ENOMEM (too few free pages) or CQ_ERANGE (a negative count, a
+ * sequence longer than max_pages, an id in its table out of range, more tokens than
+ * n_slots) the map stays as it was and every slot is -1.  `workspace`:
+ * cq_pages_workspace_bytes, 16-byte aligned. */
+int cq_pages_append(const cq_kv_pages* pages, const cq_page_map* map, const int32_t* d_add, int32_t* d_slots,
+                    int32_t n_slots, int32_t* d_status, void* workspace, void* stream);
+size_t cq_pages_workspace_bytes(const cq_page_map* map);
+
+/* Sequence d_seq[i] keeps its first d_keep[i] tokens (d_keep NULL: none); pages past
+ * them are given back, and their table entries set to -1; n is at most 1024.  Nothing
+ * changes where it has no more than that.  d_status[i] (n ints): CQ_OK; CQ_ERANGE: an id outside [0,
+ * n_seqs), a negative count, a len out of range; CQ_EINVAL: an earlier entry names the
+ * sequence too. */
+int cq_pages_trim(const cq_page_map* map, const int32_t* d_seq, const int32_t* d_keep, int32_t n, int32_t* d_status,
+                  void* stream);
+
+/* Moves the used pages together: with U pages in use, the k-th free page below U
+ * takes the contents of the k-th used page at or above U, in every layer, and tables
+ * and counts follow.  d_remap (n_pages ints): the new number of each page, -1 for one
+ * that was free.  d_status (4 ints): CQ_OK, U, pages moved, 0.  `workspace` as for
+ * cq_pages_append. */
+int cq_pages_compact(const cq_kv_pages* pages, const cq_page_map* map, int32_t* d_remap, int32_t* d_status,
+                     void* workspace, void* stream);
+
+/* Copies page d_src[i] of `src` to page d_dst[i] of `dst` (the same pool, or one of
+ * the same kv_dtype, layers, heads, head_dim and page_tokens), all layers; no
+ * counts change.  d_status[i] (n ints): CQ_OK; CQ_ERANGE: an id outside its pool;
+ * CQ_EINVAL: another pair has the same d_dst, or, within one pool, has it as its
+ * d_src (a page onto itself is CQ_OK).  Refused pairs are not copied.  n is at most
+ * 4096.  Two pools that differ do not overlap in memory. */
+int cq_pages_copy(const cq_kv_pages* src, const cq_kv_pages* dst, const int32_t* d_src, const int32_t* d_dst, int32_t n,
+                  int32_t* d_status, void* stream);
+
+/* Rows of K and V (n_tokens rows of n_kv_heads * head_dim halves, row_stride halves
+ * apart, a multiple of 8, 16-byte aligned) into the slots of one layer; a one-byte
+ * pool quantizes each (token, head) row as CQ_KV_INT8 / CQ_KV_FP8 do.  Rows whose
+ * slot lies outside [0, n_pages * page_tokens) are left out; no slot is named twice. */
+int cq_paged_kv_store(const cq_kv_pages* pages, int32_t layer, const void* k, const void* v, int64_t row_stride,
+                      const int32_t* d_slots, int32_t n_tokens, void* stream);
+/* The reverse: the rows of the slots as fp16 (one-byte: half(value * scale)); a row
+ * whose slot lies outside the pool is left as it was. */
+int cq_paged_kv_load(const cq_kv_pages* pages, int32_t layer, void* k, void* v, int64_t row_stride,
+                     const int32_t* d_slots, int32_t n_tokens, void* stream);
+
+/* Decode attention of one layer for a batch whose sequences share a prefix, which is
+ * read once for all of them: row b of q (n_heads * head_dim halves, q_stride halves
+ * apart, a multiple of 8) attends over positions [0, *d_prefix_len) of the pages in
+ * d_prefix_table (prefix_pages ints) of `prefix` and over positions [*d_start,
+ * d_len[b]) of the pages in row b of d_table (max_pages ints a row) of `own`:
+ * out[b][h] = softmax(q_h . K^T / sqrt(head_dim)) V over both, kv head h / (n_heads /
+ * n_kv_heads).  d_start NULL: 0.  Sequences forked from one prompt: `prefix` and `own`
+ * are the same pool, d_prefix_table the row of any of them, d_start = d_prefix_len.
+ * A row that sees no position is zeros; a row with d_len[b] < 0 is left as it was.
+ * Lengths past what a table row holds are cut there; pages outside the pool are not
+ * seen.  batch in [0, 1024], up to 16 query heads per kv head; q and out 16-byte
+ * aligned and apart.  `workspace`: cq_prefix_attention_workspace_bytes, 16-byte aligned,
+ * of its own for calls that may overlap. */
+int cq_prefix_attention_decode(const void* q, int64_t q_stride, void* out, int64_t out_stride, const cq_kv_pages* prefix,
+                               const int32_t* d_prefix_table, int32_t prefix_pages, const int32_t* d_prefix_len,
+                               const cq_kv_pages* own, const int32_t* d_table, int32_t max_pages,
+                               const int32_t* d_start, const int32_t* d_len, int32_t batch, int32_t layer,
+                               int32_t n_heads, void* workspace, void* stream);
+size_t cq_prefix_attention_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+
 /* Dequantise rows of a quantized matrix to fp32 with the device unpacking
  * path of the GEMVs (q * fp16 scale): out[rows][cols].  Test hook for the
  * bit-exact unpack check; no counterpart in the reference. */

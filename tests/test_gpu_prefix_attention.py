@@ -1,0 +1,388 @@
+"""GPU tests of the batch attention over a shared prefix (cq_prefix_attention_decode)
+against the formula in 64 bits.
+
+Tolerance, per output element, with w the softmax weights and A = sum w |v|:
+  the output's rounding to fp16        2^-11 |out| + 2^-25
+  each weight's rounding to fp16       2^-11 A, and 2^-25 |v| for each key whose
+                                       exponential lies in fp16's subnormals (times r
+                                       for one-byte V: see the kernel), over l >= 1
+  scores and sums in fp32              2^-14 A (|s| log2(e) 2^-23 and the products'
+                                       2^-24 sqrt(hd) |q| |k|, below 2^-15 at the
+                                       scores of up to 60 used here)"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import cuqwen_amd as cq
+from tests.conftest import tiny_config
+from tests.gpu_util import Pool
+from tests.pages_util import DevicePool, Hip, ceil
+
+pytestmark = pytest.mark.gpu
+L = cq.lib
+KVS = [cq.KV_FP16, cq.KV_INT8, cq.KV_FP8]
+
+
+@pytest.fixture
+def g():
+    p = Pool()
+    yield p
+    p.close()
+
+
+class Case:
+    """A batch of forked sequences (one pool, shared pages first) or, with `apart`, a prefix in a pool of
+    its own and tables that hold only the sequences' own tokens."""
+
+    def __init__(self, g, seed, kv, heads, n_kv, hd, page, prefix, own, form="own", apart=False, layers=1, qscale=1.5):
+        rng = self.rng = np.random.default_rng(seed)
+        self.g, self.kv, self.heads, self.n_kv, self.hd, self.page, self.prefix = g, kv, heads, n_kv, hd, page, prefix
+        self.batch = len(own)
+        self.layer = layers - 1
+        full = 0 if apart else prefix // page
+        self.start = 0 if apart else prefix
+        self.lens = [n if n < 0 else self.start + n for n in own]
+        more = [max(ceil(max(n, 0), page) - full, 0) for n in self.lens]
+        n_pre = ceil(prefix, page)
+        total = (0 if apart else full + (n_pre > full)) + sum(more) + 2
+        ids = rng.permutation(total).tolist()
+        shared, ids = ids[:full], ids[full:]
+        self.rows = []
+        for n in more:
+            self.rows.append(shared + ids[:n])
+            ids = ids[n:]
+        self.pool = DevicePool(g, rng, kv, layers, total, page, n_kv, hd, form)
+        if apart:
+            self.pre = DevicePool(g, rng, kv, layers, n_pre + 1, page, n_kv, hd, "cache" if form == "own" else "own")
+            self.pre_row = rng.permutation(n_pre + 1)[:n_pre].tolist()
+        else:
+            self.pre = self.pool
+            self.pre_row = shared + ([ids[0]] if n_pre > full else [])
+        self.width = max([len(r) for r in self.rows] + [1]) + 1
+        self.q = (rng.standard_normal((self.batch, heads, hd)) * qscale).astype(np.float16)
+
+    def want(self):
+        """(out, tolerance); NaN rows where nothing is written."""
+        g, scale = self.heads // self.n_kv, 1 / np.sqrt(self.hd)
+        out, tol = (np.full((self.batch, self.heads, self.hd), np.nan) for _ in range(2))
+        pre = [self.pre.rows(k, self.layer, self.pre_row) if self.pre_row else np.zeros((0, self.n_kv, self.page, self.hd)) for k in (0, 1)]
+        pre = [x.transpose(1, 0, 2, 3).reshape(self.n_kv, -1, self.hd)[:, :self.prefix] for x in pre]
+        for b in range(self.batch):
+            if self.lens[b] < 0:
+                continue
+            own = []
+            for k in (0, 1):
+                x = self.pool.rows(k, self.layer, self.rows[b]) if self.rows[b] else np.zeros((0, self.n_kv, self.page, self.hd))
+                own.append(x.transpose(1, 0, 2, 3).reshape(self.n_kv, -1, self.hd)[:, self.start:max(self.lens[b], self.start)])
+            for h in range(self.heads):
+                K, V = (np.concatenate([pre[k][h // g], own[k][h // g]]) for k in (0, 1))
+                if not len(K):
+                    out[b, h] = tol[b, h] = 0
+                    continue
+                s = K @ self.q[b, h].astype(np.float64) * scale
+                p = np.exp(s - s.max())
+                w = p / p.sum()
+                out[b, h] = w @ V
+                top = np.abs(V).max() * 2   # r times the largest code: below twice the largest |v|
+                tol[b, h] = 2.0 ** -11 * np.abs(out[b, h]) + 2.0 ** -25 + (2.0 ** -11 + 2.0 ** -14) * (w @ np.abs(V)) + \
+                    2.0 ** -25 * top * len(K) / p.sum()
+        return out, tol
+
+    def put(self):
+        g, n = self.g, self.heads * self.hd
+        self.qs, self.os = n + 8, n + 24
+        q = np.zeros((self.batch, self.qs), np.float16)
+        q[:, :n] = self.q.reshape(self.batch, n)
+        table = np.full((self.batch, self.width), -1, np.int32)
+        for b, r in enumerate(self.rows):
+            table[b, :len(r)] = r
+        self.host_table = table
+        self.d = dict(q=g.put(q), table=g.put(table), pre=g.i32(self.pre_row + [-1]), plen=g.i32(self.prefix), start=g.i32(self.start),
+                      lens=g.i32(self.lens))
+        self.out = g.empty(self.batch * self.os * 2)
+        self.ws = g.empty(L.cq_prefix_attention_workspace_bytes(self.batch, self.heads, self.n_kv, self.hd))
+        return self
+
+    def call(self, stream=None, start="start"):
+        d = self.d
+        cq.check(L.cq_prefix_attention_decode(d["q"], self.qs, self.out.ptr, self.os, self.pre.arg(), d["pre"], len(self.pre_row) + 1,
+                                              d["plen"], self.pool.arg(), d["table"], self.width, d[start] if start else None, d["lens"],
+                                              self.batch, self.layer, self.heads, self.ws.ptr, stream))
+
+    def run(self):
+        self.put()
+        self.out.upload(np.full((self.batch, self.os), -9, np.float16))
+        self.call(start="start" if self.start else None)
+        return self.out.to_array(np.float16, (self.batch, self.os)).astype(np.float64)
+
+    def check(self, got=None):
+        got = self.run() if got is None else got
+        n = self.heads * self.hd
+        want, tol = (x.reshape(self.batch, n) for x in self.want())
+        assert np.all(got[:, n:] == -9)
+        gone = np.isnan(want)
+        assert np.all(got[:, :n][gone] == -9)
+        err = np.abs(got[:, :n] - want)[~gone]
+        assert np.all(np.isfinite(got[:, :n])), "not finite"
+        over = err - tol[~gone]
+        assert err.size == 0 or over.max() <= 0, f"off by {err[over.argmax()]:.3g}, tolerance {tol[~gone][over.argmax()]:.3g}"
+
+
+SHAPES = [(14, 2, 64), (28, 4, 128), (4, 4, 64), (16, 1, 128), (5, 5, 128), (40, 8, 128)]
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("heads,n_kv,hd", SHAPES)
+def test_head_layouts(g, kv, heads, n_kv, hd):
+    Case(g, heads, kv, heads, n_kv, hd, 64, 130, [1, 70, 33], layers=2).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("page", [32, 64, 256])
+@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 64, 255, 256, 257, 1000])
+def test_prefix_lengths(g, kv, page, prefix):
+    Case(g, prefix + page, kv, 6, 2, 64, page, prefix, [0, 1, 31, 32, 65, -1, 300]).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("form", ["own", "wide", "cache"])
+def test_prefix_in_a_pool_of_its_own(g, kv, form):
+    Case(g, 3, kv, 14, 2, 64, 64, 333, [0, 1, 100, 64, -5, 7], form, apart=True, layers=3).check()
+    Case(g, 4, kv, 4, 2, 128, 32, 0, [0, 5, 64, -1], form, apart=True).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("batch", [1, 2, 3, 5, 9, 10, 16, 19, 33, 37, 64, 74, 130])
+def test_batches(g, kv, batch):
+    rng = np.random.default_rng(batch)
+    Case(g, batch, kv, 14, 2, 64, 32, 700, rng.integers(0, 90, batch).tolist()).check()
+    Case(g, batch, kv, 7, 1, 128, 64, 999, rng.integers(0, 60, batch).tolist()).check()
+
+
+def test_largest_batch(g):
+    rng = np.random.default_rng(1)
+    Case(g, 1, cq.KV_FP16, 2, 1, 64, 32, 100, rng.integers(0, 40, 1024).tolist()).check()
+    Case(g, 2, cq.KV_INT8, 2, 2, 64, 32, 2500, rng.integers(0, 40, 1023).tolist()).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+def test_long_prefix_and_ragged_own(g, kv):
+    Case(g, 5, kv, 14, 2, 64, 128, 9001, [3000, 1, 0, 513, 64, 31, 2, 1999]).check()
+    Case(g, 6, kv, 7, 1, 128, 64, 20011, [7] * 40).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+def test_only_own_tokens_or_nothing(g, kv):
+    Case(g, 7, kv, 4, 2, 64, 32, 0, [0, 0, 0]).check()
+    Case(g, 8, kv, 4, 2, 64, 32, 0, [5000, 0, 1]).check()
+    Case(g, 9, kv, 4, 2, 64, 32, 0, [-1, -1]).check()
+    Case(g, 10, kv, 4, 2, 64, 32, 77, [-1, -3]).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+def test_sharp_and_large_scores(g, kv):
+    """Scores of some tens: the weights of one key or two decide."""
+    Case(g, 11, kv, 14, 2, 64, 64, 500, [20, 100, 3], qscale=12).check()
+
+
+@pytest.mark.parametrize("kv", [cq.KV_INT8, cq.KV_FP8])
+@pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -20, 2.0 ** 8])
+def test_small_and_large_scales_of_v(g, kv, size):
+    """One-byte V whose scales would drive fp16 products into the subnormals, or rows of very different size."""
+    c = Case(g, 12, kv, 7, 1, 64, 32, 400, [50, 3, 77])
+    for s in c.pool.scales[1:]:
+        s *= np.float32(size) * np.where(c.rng.random(s.shape) < 0.5, 1, 2.0 ** -9).astype(np.float32)
+    c.pool.upload()
+    got = c.run()
+    n = c.heads * c.hd
+    want, tol = (x.reshape(c.batch, n) for x in c.want())
+    assert np.all(np.abs(got[:, :n] - want) <= tol)
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("what", [np.nan, np.inf, -65504.0])
+def test_anything_may_lie_behind_the_lengths(g, kv, what):
+    """Slots past a prefix and past a sequence, before its start, and pages that nobody names."""
+    c = Case(g, 13, kv, 14, 2, 64, 64, 100, [20, 29, 1, 0, 64])
+    ref = c.want()
+    seen = np.zeros((c.pool.n_pages, c.page), bool)
+    for t in range(c.prefix):
+        seen[c.pre_row[t // c.page], t % c.page] = True
+    for row, n in zip(c.rows, c.lens):
+        for t in range(c.start, n):
+            seen[row[t // c.page], t % c.page] = True
+    for k in (0, 1):
+        at = c.pool.at[0][~seen.any(-1)]
+        for p, t in zip(*np.nonzero(~seen)):
+            at = c.pool.at[0, p]
+            for h in range(c.n_kv):
+                o = at[h] + c.pool.offsets(k)[t]
+                if kv == cq.KV_FP16:
+                    c.pool.host[k][o] = what
+                else:
+                    c.pool.host[k][o] = 127 if kv == cq.KV_FP8 else -128   # E4M3: the NaN code
+                    c.pool.scales[k][at[h] // c.hd + t] = what
+    c.pool.upload()
+    got = c.run()
+    n = c.heads * c.hd
+    want, tol = (x.reshape(c.batch, n) for x in ref)
+    assert np.all(np.abs(got[:, :n] - want) <= tol)
+
+
+def test_infinities_and_nan_that_are_seen(g):
+    """A NaN or an infinite score among the visible keys shows in the rows that see it, and only there."""
+    c = Case(g, 14, cq.KV_FP16, 4, 2, 64, 32, 64, [10, 12, 3])
+    p, t = c.rows[1][2], 3           # an own token of sequence 1, kv head 1
+    c.pool.host[1][c.pool.at[0, p, 1] + c.pool.offsets(1)[t]] = np.nan
+    c.pool.upload()
+    got = c.run()[:, :c.heads * c.hd].reshape(c.batch, c.heads, c.hd)
+    assert np.isnan(got[1, 2:]).all() and np.isfinite(got[1, :2]).all() and np.isfinite(got[[0, 2]]).all()
+    c.pool.host[1][c.pool.at[0, p, 1] + c.pool.offsets(1)[t]] = 0
+    c.pool.host[0][c.pool.at[0, c.pre_row[0], 0] + c.pool.offsets(0)[5]] = np.inf   # a prefix key of kv head 0: scores of +-inf or NaN
+    c.pool.upload()
+    got = c.run()[:, :c.heads * c.hd].reshape(c.batch, c.heads, c.hd)
+    assert np.isnan(got[:, :2]).any(-1).all() and np.isfinite(got[:, 2:]).all()
+
+
+def test_pages_outside_the_pool_are_not_seen(g):
+    for batch in (3, 40):
+        c = Case(g, 15, cq.KV_FP16, 14, 2, 64, 32, 200, [40, 70, 33] + [20] * (batch - 3))
+        c.put()
+        table = c.host_table.copy()
+        table[1, 7], table[0, 6] = c.pool.n_pages, -2 ** 31     # sequence 1: positions 224..255; sequence 0: 192..223
+        pre = list(c.pre_row)
+        pre[2], pre[4] = 2 ** 31 - 1, -1                        # prefix positions 64..95, 128..159
+        c.d["table"], c.d["pre"] = g.put(table), g.i32(pre + [-1])
+        c.out.upload(np.full((c.batch, c.os), -9, np.float16))
+        c.call()
+        got = c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64)[:, :c.heads * c.hd]
+        scale, grp = 1 / np.sqrt(c.hd), c.heads // c.n_kv
+        for b in range(3):
+            for h in range(c.heads):
+                K, V = [], []
+                for t in range(c.prefix):
+                    if t // 32 not in (2, 4):
+                        K.append((c.pre_row[t // 32], t % 32))
+                for t in range(c.prefix, c.lens[b]):
+                    if not (b == 1 and t // 32 == 7) and not (b == 0 and t // 32 == 6):
+                        K.append((c.rows[b][t // 32], t % 32))
+                pid, tok = (np.array(x) for x in zip(*K))
+                k, v = (c.pool.rows(i, 0, pid)[np.arange(len(pid)), h // grp, tok] for i in (0, 1))
+                s = k @ c.q[b, h].astype(np.float64) * scale
+                p = np.exp(s - s.max())
+                w = p / p.sum()
+                tol = 2.0 ** -11 * np.abs(w @ v) + 2.0 ** -24 + (2.0 ** -11 + 2.0 ** -14) * (w @ np.abs(v)) + \
+                    2.0 ** -24 * np.abs(v).max() * len(k) / p.sum()
+                assert np.all(np.abs(got[b, h * c.hd:(h + 1) * c.hd] - w @ v) <= tol), (batch, b, h)
+
+
+def test_lengths_are_cut_at_the_tables(g):
+    """A prefix length, a sequence length and a start past what the tables hold, or below zero."""
+    c = Case(g, 16, cq.KV_INT8, 4, 2, 64, 32, 96, [10, 20, 32])
+    ref = c.run()
+    c.d["plen"] = g.i32(-4)
+    c.d["start"] = g.i32(-7)          # everything from position 0 on, by each sequence's own table
+    c.call()
+    got = c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64)
+    want, tol = c.want()
+    n = c.heads * c.hd
+    assert np.all(np.abs(got[:, :n] - want.reshape(c.batch, n)) <= tol.reshape(c.batch, n))
+    assert np.all(np.abs(ref[:, :n] - want.reshape(c.batch, n)) <= tol.reshape(c.batch, n))
+    c = Case(g, 17, cq.KV_FP16, 4, 2, 64, 32, 96, [32, 32], apart=True)
+    c.put()
+    c.d["plen"], c.d["lens"] = g.i32(2 ** 31 - 1), g.i32([2 ** 31 - 1, 2 ** 31 - 1])
+    c.out.upload(np.full((c.batch, c.os), -9, np.float16))
+    c.call(start=None)                # the entries behind are -1: nothing there is seen
+    c.check(c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64))
+    c.d["start"] = g.i32(2 ** 31 - 1)
+    c.call()                          # no own position left
+    c.lens = [0, 0]
+    c.check(c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64))
+
+
+def test_same_bits_on_every_call(g):
+    """Fixed order of all sums: two calls, and a call with a workspace full of NaN, agree bit for bit."""
+    c = Case(g, 18, cq.KV_FP16, 28, 4, 128, 64, 1500, [100, 3, 0, 40, 77] * 8)
+    a = c.run()
+    c.ws.upload(np.full(c.ws.nbytes // 2, np.nan, np.float16))
+    c.call(start="start")
+    b = c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64)
+    assert np.array_equal(a, b)
+    c.check(b)
+
+
+@pytest.mark.parametrize("kv", KVS)
+def test_captured_with_growing_lengths(g, kv):
+    """One graph, replayed as the sequences grow; eager calls of the same state between the replays."""
+    c = Case(g, 19, kv, 14, 2, 64, 64, 300, [200, 40, 90, 33, 64, 1])
+    c.put()
+    c.out.upload(np.full((c.batch, c.os), -9, np.float16))
+    hip = Hip()
+    stream = hip.stream()
+    cq.synchronize()
+    graph = hip.capture(stream, lambda: c.call(stream))
+    full = list(c.lens)
+    for cut in (190, 100, 0, 33):
+        c.lens = [max(n - cut, c.start) for n in full]
+        new = np.array(c.lens, np.int32)
+        cq.check(L.cq_memcpy_h2d(c.d["lens"], new.ctypes.data, new.nbytes))
+        hip.launch(graph, stream)
+        hip.wait(stream)
+        got = c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64)
+        c.check(got)
+        c.out.upload(np.full((c.batch, c.os), -9, np.float16))
+        c.call()
+        assert np.array_equal(c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64), got)
+    hip.drop(stream, [graph])
+
+
+def test_two_streams_with_workspaces_of_their_own(g):
+    hip = Hip()
+    streams = [hip.stream(), hip.stream()]
+    cases = [Case(g, 20 + i, cq.KV_FP16, 14, 2, 64, 32, 500 + i, [9, 70, 3, 40 + i]).put() for i in range(2)]
+    for c in cases:
+        c.out.upload(np.full((c.batch, c.os), -9, np.float16))
+    cq.synchronize()
+    for _ in range(5):
+        for c, s in zip(cases, streams):
+            c.call(s)
+    for s in streams:
+        hip.wait(s)
+    for c in cases:
+        c.check(c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64))
+    for s in streams:
+        hip.drop(s)
+
+
+def test_prefix_is_a_states_own_cache(g):
+    """The prompt that cq_prefill left in a state, read in place as the prefix of a batch."""
+    cfg = tiny_config(max_seq_len=544)
+    for kv in KVS:
+        w = cq.synth_weights(cfg, 5)
+        st = cq.State(cfg, w, kv_dtype=kv)
+        st.prefill(list(range(1, 152)))
+        c = Case(g, 22, kv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, 32, 160, [5, 40, 0, 32], apart=True, layers=2)
+        view = st.kv_pages(32)
+
+        class View:   # the prefix's values as the state gives them out
+            page_ids = None
+
+            def arg(self):
+                return ctypes.byref(view)
+
+            def rows(self, kind, layer, ids):
+                x = np.stack([st.kv_read(layer, h, kind, 160) for h in range(cfg.n_kv_heads)]).astype(np.float64)
+                return x.reshape(cfg.n_kv_heads, 5, 32, cfg.head_dim).transpose(1, 0, 2, 3)[ids]
+
+        c.pre, c.pre_row, c.prefix = View(), [0, 1, 2, 3, 4], 151
+        if kv == cq.KV_FP16:
+            c.check()
+        else:   # kv_read rounds value * scale to fp16: 2^-11 of each key's products and of each v
+            got = c.run()[:, :c.heads * c.hd]
+            want, tol = (x.reshape(c.batch, -1) for x in c.want())
+            k = np.abs(np.stack([c.pre.rows(0, 1, [0, 1, 2, 3, 4])])).max()
+            slack = 2.0 ** -11 * (1 + 2 * k * np.abs(c.q).sum(-1).max() / np.sqrt(c.hd))
+            assert np.all(np.abs(got - want) <= tol + slack * np.abs(c.pre.rows(1, 1, [0, 1, 2, 3, 4])).max())
+        st.free()
+        w.free()
