@@ -7,12 +7,14 @@
 // in pieces: each piece of keys leaves (m, l, O) in fp32, and a second launch joins the
 // pieces of a row by the log-sum-exp rule.
 //
-// Work: 32-key tiles of (item, tile), an item being (kv head, 16 query rows) of the
-// prefix or (sequence, kv head) of the own part.  All tiles of all items form one
-// list that the waves of the grid share evenly (share_of), wherever item borders fall, from the
-// lengths found on the device: lengths may be ragged, and a captured launch serves
-// other lengths.  Wave w's piece of item i is stored in slot w + i (either w or i grows from one piece to the next, so slots
-// differ), and the joining launch finds a row's pieces by the same arithmetic.
+// Work of stage 1, whose grid is one block per CU: the steps (a few 32-key tiles) of
+// all items of the prefix, an item being (kv head, block of query rows), form one
+// list that the blocks share evenly, and the tiles of all (sequence, kv head) items
+// of the own part one that the waves share evenly (share_of), wherever item borders
+// fall, from the lengths found on the device: lengths may be ragged, and a captured
+// launch serves other lengths.  Worker w's piece of item i is stored in slot w + i
+// (either w or i grows from one piece to the next, so slots differ), and the joining
+// launch finds a row's pieces by the same arithmetic.
 #include "cq_attention.h"
 #include "cq_pages.h"
 
@@ -25,7 +27,7 @@ namespace {
 
 constexpr int kPxWaves = 8, kPxThreads = kPxWaves * kWave;
 constexpr int kPxBlocks = kNumCUs;                    // one block per CU
-constexpr int kPxListWaves = kPxBlocks * kPxWaves;    // W of the own list
+constexpr int kPxListWaves = kPxBlocks * kPxWaves;    // workers of the own list
 constexpr int kPxMaxBatch = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -46,7 +48,7 @@ struct PxArgs {
   int64_t* plan;                  // [batch + 1] own tiles before each sequence, then the prefix's tiles
   float* own_o;                   // [slot][16][HD]
   float* own_ml;                  // [slot][16][2]
-  float* pre_o;
+  float* pre_o;                   // [slot][rows of a block][HD]
   float* pre_ml;
 };
 
@@ -58,6 +60,21 @@ __device__ __forceinline__ void share_of(int w, int64_t F, int W, int64_t* first
 }
 // The worker that has tile x.
 __device__ __forceinline__ int worker_of(int64_t x, int64_t F, int W) { return (int)(F <= W ? x : ((x + 1) * W - 1) / F); }
+
+// Largest of v over the four lanes that share a column (lane % 16).  The two results
+// of a swap go through variables: a bit cast of an element of the builtin's vector
+// reads its first element whatever the index.
+__device__ __forceinline__ float px_col_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t x = __float_as_uint(fmaxf(__uint_as_float(a0), __uint_as_float(a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
+}
+// One v_max3_f32 (left to the compiler, which knows the wait states of matrix results).
+__device__ __forceinline__ float px_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // Positions that a table of n pages holds, and the length cut there.
 __device__ __forceinline__ int cut_len(int len, int pages, int shift) {
@@ -171,8 +188,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
   for (int a = 0; a < 2; ++a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) mn = fmaxf(mn, s[a][i]);
-  mn = fmaxf(mn, __shfl_xor(mn, 16, kWave));
-  mn = fmaxf(mn, __shfl_xor(mn, 32, kWave));
+  mn = px_col_max(mn);
   float rn = st.r;
   if constexpr (F != CQ_KV_FP16) {
     float vm = 0.f;
@@ -180,9 +196,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 4; ++i) vm = fmaxf(vm, t.vs[a][i]);
-    vm = fmaxf(vm, __shfl_xor(vm, 16, kWave));
-    vm = fmaxf(vm, __shfl_xor(vm, 32, kWave));
-    rn = fmaxf(rn, __uint_as_float(__float_as_uint(vm) & 0x7f800000u));
+    rn = fmaxf(rn, __uint_as_float(__float_as_uint(px_col_max(vm)) & 0x7f800000u));
   }
   if (__any(mn > st.m || rn > st.r)) {
     const float alpha = mn == st.m ? 1.f : __builtin_amdgcn_exp2f((st.m - mn) * c2);
@@ -195,63 +209,561 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
   }
   const float mm = st.m == -INFINITY ? 0.f : st.m * c2;   // no valid key yet: the masked ones give 0
   const float ri = F != CQ_KV_FP16 ? 1.f / st.r : 1.f;
-  h8_t pb;
+  // each weight in two fp16 parts, 22 bits: the matrix units idle here anyway
+  h8_t pb, pc;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float p = __builtin_amdgcn_exp2f(fmaf(s[a][i], c2, -mm));
       st.l += p;
-      // fp16: half a step of 2^-11 of each weight, while the sum keeps them whole
-      pb[a * 4 + i] = (_Float16)(F != CQ_KV_FP16 ? p * (t.vs[a][i] * ri) : p);
+      const float x = F != CQ_KV_FP16 ? p * (t.vs[a][i] * ri) : p;
+      pb[a * 4 + i] = (_Float16)x;
+      pc[a * 4 + i] = (_Float16)(x - (float)pb[a * 4 + i]);
     }
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) st.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(px_operand<F>(t.v, dt, magic), pb, st.o[dt], 0, 0, 0);
+  for (int dt = 0; dt < DT; ++dt) {
+    const h8_t v = px_operand<F>(t.v, dt, magic);
+    st.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb, st.o[dt], 0, 0, 0);
+    st.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pc, st.o[dt], 0, 0, 0);
+  }
 }
 
-// Tiles [ta, tb) of one cache for the rows q[r0 .. r0 + rows) of a kv head; the
-// state goes to (o, ml).
+// Tiles ta, ta + step, ... < tb of one cache for the rows q[r0 .. r0 + rows) of a kv
+// head: the wave's state, m in log2 units and O in the values' own units.
 template <int HD, int F>
-__device__ __forceinline__ void px_piece(const PxArgs& a, const PxKV& kv, int kvh, int r0, int rows, int lo, int hi, int ta, int tb,
-                                         float* o, float* ml, int lane) {
+__device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, const PxKV& kv, int kvh, int r0, int rows, int lo, int hi, int ta,
+                                       int tb, int step, int lane) {
   constexpr int KK = HD / 32, DT = HD / 16;
   const int h = lane & 15, j = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);
   const uint32_t magic = vgpr_const(0x64646464u);
   PxTile<HD, F> A, B;
-  px_load<HD, F>(A, kv, ta, lo, hi, true, lane);
+  px_load<HD, F>(A, kv, ta, lo, hi, ta < tb, lane);
   h8_t qb[KK];
   const int r = r0 + min(h, rows - 1), b = r / a.g;
   const _Float16* q = a.q + b * a.q_stride + (kvh * a.g + (r - b * a.g)) * HD;
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) qb[kk] = __builtin_bit_cast(h8_t, load_u4(q + kk * 32 + j * 8));
-  PxState<HD> st;
   st.m = -INFINITY;
   st.l = 0.f;
   st.r = 0x1p-100f;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) st.o[dt] = f4_t{0.f, 0.f, 0.f, 0.f};
-  for (int ti = ta; ti < tb; ti += 2) {
-    px_load<HD, F>(B, kv, ti + 1, lo, hi, ti + 1 < tb, lane);
+  for (int ti = ta; ti < tb; ti += 2 * step) {
+    px_load<HD, F>(B, kv, ti + step, lo, hi, ti + step < tb, lane);
     px_attend<HD, F>(A, qb, st, c2, lane, magic);
-    if (ti + 1 >= tb) break;
-    px_load<HD, F>(A, kv, ti + 2, lo, hi, ti + 2 < tb, lane);
+    if (ti + step >= tb) break;
+    px_load<HD, F>(A, kv, ti + 2 * step, lo, hi, ti + 2 * step < tb, lane);
     px_attend<HD, F>(B, qb, st, c2, lane, magic);
   }
+  st.m *= c2;
   st.l += __shfl_xor(st.l, 16, kWave);
   st.l += __shfl_xor(st.l, 32, kWave);
-  if (h < rows) {
+  if constexpr (F != CQ_KV_FP16) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4_t*>(o + h * HD + dt * 16 + 4 * j) = F != CQ_KV_FP16 ? st.o[dt] * st.r : st.o[dt];
+    for (int dt = 0; dt < DT; ++dt) st.o[dt] *= st.r;
+  }
+}
+
+// The own part's piece: one wave's.
+template <int HD, int F>
+__device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, int kvh, int b, int lo, int hi, int ta, int tb, float* o,
+                                             float* ml, int lane) {
+  const int h = lane & 15, j = lane >> 4;
+  PxState<HD> st;
+  px_run<HD, F>(st, a, kv, kvh, b * a.g, a.g, lo, hi, ta, tb, 1, lane);
+  if (h < a.g) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) *reinterpret_cast<f4_t*>(o + h * HD + dt * 16 + 4 * j) = st.o[dt];
     if (j == 0) {
-      ml[2 * h] = st.m * c2;   // log2 units from here on
+      ml[2 * h] = st.m;
       ml[2 * h + 1] = st.l;
     }
   }
 }
 
-template <int HD, int F>
-__global__ __launch_bounds__(kPxThreads) void px_stage1(const PxArgs a) {
+// How a block attends over the prefix with ROWS query rows.  Up to 32 rows every wave
+// takes 16 of them over tiles of its own in registers (the K / V operands feed one
+// instruction each, and HBM is what bounds it); beyond that 32 rows over tiles in LDS,
+// which the row groups share.  KH waves share a row group's keys.
+template <int HD, int F, int ROWS>
+struct PxForm {
+  static constexpr bool LDS = ROWS > 32;
+  static constexpr int WR = LDS ? 32 : 16;              // rows of a wave
+  static constexpr int RG = ROWS / WR, KH = kPxWaves / RG;
+  static constexpr int TPW = !LDS ? 1 : KH == 1 ? 2 : KH == 2 ? (HD == 128 && F != CQ_KV_FP16 ? 1 : 2) : (HD == 64 ? 2 : 1);
+  static constexpr int TPS = KH * TPW;                  // tiles of a step
+  static constexpr int TILE = kTileKeys * HD;           // halves of K (or V) per tile
+  static constexpr int STAGE = 2 * TPS * TILE;          // halves: K tiles, then V tiles
+  // LDS slots: three (requests two steps ahead) where they fit 96 KB, else two
+  static constexpr int NS = F == CQ_KV_FP16 && 3 * STAGE * 2 <= 96 * 1024 ? 3 : 2;
+  static constexpr int DT = HD / 16, CG = WR / 16;
+  static constexpr int STATE = 4 + 4 * DT * CG;         // floats of one lane's softmax state: (m, l) of up to two slices, O
+  // halves of LDS: the stages, over them the states of the other key groups
+  static constexpr int SM = LDS ? std::max(NS * STAGE, (KH - 1) * RG * kWave * STATE * 2) : kPxWaves * kWave * STATE * 2;
+  static constexpr int SCL = LDS && F != CQ_KV_FP16 ? (NS + 3) * TPS * kTileKeys : 1;   // K scales per slot, V scales three steps
+};
+
+// Tiles [tb, te) of the prefix for up to 32 rows.
+template <int HD, int F, int ROWS>
+__device__ __forceinline__ void px_stream_piece(const PxArgs& a, float* sm, int kvh, int r0, int R, int lp, int tb, int te, float* o,
+                                                float* ml) {
+  using P = PxForm<HD, F, ROWS>;
+  constexpr int DT = HD / 16, RG = P::RG, KH = P::KH;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int rg = wave % RG, kg = wave / RG, rw = r0 + rg * 16;
+  const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table};
+  PxState<HD> st;
+  px_run<HD, F>(st, a, kv, kvh, min(rw, R - 1), max(min(16, R - rw), 1), 0, lp, tb + kg, rw < R ? te : tb, KH, lane);
+  // the key groups' states through LDS: [wave][1 + DT][lane] of (m, l, -, -), O
+  static_assert(P::STATE == 4 * (1 + DT), "LDS holds the states");
+  f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * (1 + DT) * kWave + lane;
+  __syncthreads();
+  *w = f4_t{st.m, st.l, 0.f, 0.f};
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) w[(1 + dt) * kWave] = st.o[dt];
+  __syncthreads();
+  // a wave joins DT / KH of its row group's dim tiles (KH = 8 with DT = 4: half of the waves)
+  const int h = lane & 15, j = lane >> 4;
+  if (rw + h >= R) return;
+  const f4_t* s = reinterpret_cast<const f4_t*>(sm) + lane;
+  float m1[KH], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int k = 0; k < KH; ++k) {
+    m1[k] = s[(k * RG + rg) * (1 + DT) * kWave][0];
+    M = fmaxf(M, m1[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < KH; ++k) {
+    m1[k] = m1[k] == M ? 1.f : __builtin_amdgcn_exp2f(m1[k] - M);
+    L += s[(k * RG + rg) * (1 + DT) * kWave][1] * m1[k];
+  }
+  for (int dt = kg; dt < DT; dt += KH) {
+    f4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KH; ++k) O += s[((k * RG + rg) * (1 + DT) + 1 + dt) * kWave] * m1[k];
+    *reinterpret_cast<f4_t*>(o + (rg * 16 + h) * HD + dt * 16 + 4 * j) = O;
+  }
+  if (kg == 0 && j == 0) {
+    ml[2 * (rg * 16 + h)] = M;
+    ml[2 * (rg * 16 + h) + 1] = L;
+  }
+}
+
+// Tiles [tb, te) of the prefix for 64, 128 or 256 rows: the prefill attention's loop
+// over pages, without its causal limits.
+template <int HD, int F, int ROWS>
+__device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem, float* scl, int kvh, int r0, int R, int lp, int tb, int te,
+                                                float* o_out, float* ml_out) {
+  using P = PxForm<HD, F, ROWS>;
+  constexpr bool KV8 = F != CQ_KV_FP16;
+  constexpr int KK = HD / 32, DT = HD / 16, CG = P::CG, RG = P::RG, KH = P::KH, TPW = P::TPW, TPS = P::TPS, ST = 2 * TPW;
+  constexpr int TILE = P::TILE, NS = P::NS, ES = KV8 ? 1 : 2;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int h = lane & 15, j = lane >> 4;
+  const int rg = wave % RG, kg = wave / RG, rw = r0 + rg * 32;
+  const bool idle = rw >= R;   // no rows: the wave only helps to stage
+  const int lim = min(lp, te * kTileKeys), s5 = a.pre.shift - 5;
+  const int n_steps = (te - tb + TPS - 1) / TPS;
+  const float c2 = kLog2e / sqrtf((float)HD);
+  const int64_t head = a.pre_layer + kvh * a.pre.head_stride;
+
+  // Pages of a step's tiles, one step ahead of the requests that need them; tiles past
+  // the range repeat its last one (and are masked).  A page outside the pool is read
+  // as page 0 and its keys masked: `bad` holds TPS bits per step, the latest lowest.
+  struct Ids { int page[TPS]; };
+  uint32_t bad = 0;
+  auto tile_at = [&](int ti) __attribute__((always_inline)) { return min(ti, te - 1); };
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    Ids r;
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < TPS; ++i) {
+      const int p = (int)load_ctl_u32(a.pre_table + (tile_at(tb + step * TPS + i) >> s5));
+      const bool ok = p >= 0 && p < a.pre.n_pages;
+      r.page[i] = ok ? p : 0;
+      b |= ok ? 0u : 1u << i;
+    }
+    bad = (bad << TPS) | b;
+    return r;
+  };
+  // element offset of tile `i` of a step whose pages are `id`
+  auto tile_off = [&](const Ids& id, int step, int i) __attribute__((always_inline)) {
+    return head + (int64_t)id.page[i] * a.pre.page_stride + (int64_t)(tile_at(tb + step * TPS + i) & ((1 << s5) - 1)) * TILE;
+  };
+  // fp16 cache: straight into LDS, 1 KB per wave instruction, no registers
+  constexpr int TB = TILE * 2 / 1024, PW = TPS * TB / kPxWaves;   // KB of a tile's K (or V); instructions per wave and step
+  static_assert(KV8 || PW * kPxWaves == TPS * TB, "whole pieces per wave");
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  const uint32_t lane16 = lane * 16;
+  auto dma = [&](const Ids& id, int step, int part) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int p = i * kPxWaves + wave;
+      // tile of the piece: i (8 KB tiles) or 2 i and 2 i + 1 (4 KB tiles)
+      const int64_t off = TB == 8 ? tile_off(id, step, i) : wave < 4 ? tile_off(id, step, i * 2 % TPS) : tile_off(id, step, (i * 2 + 1) % TPS);
+      lds_load_1k(lds0 + ((step % NS) * P::STAGE + part * TPS * TILE) * 2 + p * 1024, lane16, a.pre.kv[part] + off * 2 + p % TB * 1024);
+    }
+  };
+  // keys that are not there may hold anything: keep them out of P*V (each wave clears
+  // them in the pieces of V that it requested, once they are there)
+  auto clear_tail = [&](int step, uint32_t bits) __attribute__((always_inline)) {
+    if ((tb + (step + 1) * TPS) * kTileKeys <= lim && bits == 0) return;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int p = i * kPxWaves + wave, n = p / TB, k0 = tile_at(tb + step * TPS + n) * kTileKeys + 4 * j;
+      const int end = bits >> n & 1 ? 0 : lim;
+      h8_t* q = reinterpret_cast<h8_t*>(smem + (step % NS) * P::STAGE + TPS * TILE + p * 512 + lane * 8);
+      h8_t v = *q;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k0 + (e < 4 ? e : 12 + e) >= end) v[e] = (_Float16)0.f;
+      *q = v;
+    }
+  };
+  // one-byte cache: 16-byte pieces through registers, converted to fp16 on the way into
+  // LDS, so the codes are expanded once per block
+  constexpr int TP = TILE / 16, QL = KV8 ? (TPS * TP + kPxThreads - 1) / kPxThreads : 1;   // pieces of a tile; per thread
+  constexpr bool FULL = QL * kPxThreads == TPS * TP;   // else (one piece) the last threads have none
+  static_assert(!KV8 || FULL || QL == 1, "whole pieces per thread");
+  const uint32_t magic = vgpr_const(0x64646464u);
+  struct Pieces { u4_t w[QL]; float s[2]; };
+  constexpr int SK = TPS * kTileKeys;
+  float *scl_k = scl, *scl_v = scl + NS * SK;   // V scales come with the K of their step, so three slots
+  auto load = [&](Pieces& r, const Ids& id, int step, int part, uint32_t bits) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int c = FULL ? i * kPxThreads + threadIdx.x : min((int)threadIdx.x, TPS * TP - 1);
+      int64_t off = 0;
+#pragma unroll
+      for (int n = 0; n < TPS; ++n)
+        if (c / TP == n) off = tile_off(id, step, n);
+      r.w[i] = load_u4(a.pre.kv[part] + off + c % TP * 16);
+    }
+    if (part == 0 && threadIdx.x < SK) {
+      const int c = threadIdx.x, n = c / kTileKeys, key = tile_at(tb + step * TPS + n) * kTileKeys + c % kTileKeys;
+      int64_t off = 0;
+#pragma unroll
+      for (int i = 0; i < TPS; ++i)
+        if (n == i) off = tile_off(id, step, i);
+      off = off / HD + c % kTileKeys;
+      const bool in = key < lim && !(bits >> n & 1) && tb + step * TPS + n < te;
+      r.s[0] = in ? a.pre.scale[0][off] : 0.f;
+      r.s[1] = in ? a.pre.scale[1][off] : 0.f;
+    }
+  };
+  auto store = [&](const Pieces& r, int step, int part, uint32_t bits) __attribute__((always_inline)) {
+    _Float16* dst = smem + (step % NS) * P::STAGE + part * TPS * TILE;
+    const bool whole = F == CQ_KV_INT8 || part == 0 || ((tb + (step + 1) * TPS) * kTileKeys <= lim && bits == 0);
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int c = i * kPxThreads + threadIdx.x, q = c % TP;
+      if (!FULL && c >= TPS * TP) break;
+      // 16 bytes: the operand pieces of two instructions
+      _Float16* d = dst + (c / TP) * TILE + ((q / 64) * 128 + q % 64) * 8;
+      h8_t v[2] = {codes_to_h8<F>(u2_t{r.w[i].x, r.w[i].y}, magic), codes_to_h8<F>(u2_t{r.w[i].z, r.w[i].w}, magic)};
+      if (!whole) {   // an E4M3 code that is not there may be NaN
+        const int n = c / TP, k0 = tile_at(tb + step * TPS + n) * kTileKeys + 4 * (q % 64 / 16), end = bits >> n & 1 ? 0 : lim;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + (e < 4 ? e : 12 + e) >= end) v[0][e] = v[1][e] = (_Float16)0.f;
+      }
+      *reinterpret_cast<h8_t*>(d) = v[0];
+      *reinterpret_cast<h8_t*>(d + 512) = v[1];
+    }
+    if (part == 0 && threadIdx.x < SK) {
+      scl_k[step % NS * SK + threadIdx.x] = r.s[0];
+      scl_v[step % 3 * SK + threadIdx.x] = r.s[1];
+    }
+  };
+  // Group g = (K of step g + 1, V of step g), requested NS - 1 steps ahead.
+  Pieces pk, pv8;
+  Ids id_v = fetch(0), id_k = id_v, id_n;
+  constexpr uint32_t BITS = (1u << TPS) - 1;
+  auto request = [&](int g) __attribute__((always_inline)) {
+    if constexpr (KV8) {
+      load(pk, id_k, g + 1, 0, bad >> TPS & BITS);
+      load(pv8, id_v, g, 1, 0);
+    } else {
+      dma(id_k, g + 1, 0);
+      dma(id_v, g, 1);
+    }
+    id_v = id_k;
+    id_k = id_n;
+    id_n = fetch(g + 3);
+  };
+  // Group g in LDS for every wave (its readers' slots free since the last barrier).  The
+  // pages of step g + NS + 1 have been fetched by then.
+  auto arrive = [&](int g) __attribute__((always_inline)) {
+    if constexpr (KV8) {
+      store(pk, g + 1, 0, 0);
+      store(pv8, g, 1, bad >> (NS + 1) * TPS & BITS);
+    } else {
+      wait_vm<(NS - 2) * 2 * PW>();
+      clear_tail(g, bad >> (NS + 1) * TPS & BITS);
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    lds_barrier();
+  };
+
+  h8_t qb[CG][KK];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const int r = min(rw + cg * 16 + h, R - 1), b = r / a.g;
+    const _Float16* q = a.q + b * a.q_stride + (kvh * a.g + (r - b * a.g)) * HD;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qb[cg][kk] = __builtin_bit_cast(h8_t, load_u4(q + kk * 32 + j * 8));
+  }
+  float m[CG], l[CG], r = 0x1p-100f;   // running maximum (raw products, K scale applied), lane's sum, unit of O
+  f4_t o[DT][CG];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    m[cg] = -INFINITY;
+    l[cg] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][cg] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  typedef f4_t S_t[ST][CG];
+  auto qk = [&](S_t& s, int step) __attribute__((always_inline)) {   // S^T of the wave's tiles
+    const _Float16* kt = smem + (step % NS) * P::STAGE + kg * TPW * TILE;
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) s[st][cg] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const h8_t ka = *reinterpret_cast<const h8_t*>(kt + st * 16 * HD + (kk * 64 + lane) * 8);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) s[st][cg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[cg][kk], s[st][cg], 0, 0, 0);
+      }
+    }
+  };
+  auto scale_mask = [&](S_t& s, int step, uint32_t bits) __attribute__((always_inline)) {
+    const int t0 = tb + step * TPS + kg * TPW;   // the wave's first tile
+    if constexpr (KV8) {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const f4_t ks = *reinterpret_cast<const f4_t*>(scl_k + step % NS * SK + kg * TPW * kTileKeys + st * 16 + 4 * j);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) s[st][cg] *= ks;
+      }
+    }
+    if ((t0 + TPW) * kTileKeys > lim || bits) {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int end = bits >> (kg * TPW + st / 2) & 1 ? 0 : lim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = t0 * kTileKeys + st * 16 + 4 * j + i;
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) s[st][cg][i] = key >= end ? -INFINITY : s[st][cg][i];
+        }
+      }
+    }
+  };
+  float mn[CG], rn = r;
+  auto row_max = [&](const S_t& s, int step) __attribute__((always_inline)) {   // the running maximum with s
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      float mx = m[cg];
+#pragma unroll
+      for (int st = 0; st < ST; ++st) mx = px_max3(px_max3(mx, s[st][cg][0], s[st][cg][1]), s[st][cg][2], s[st][cg][3]);
+      mn[cg] = px_col_max(mx);
+    }
+    if constexpr (KV8) {
+      float vm = 0.f;
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const f4_t vs = *reinterpret_cast<const f4_t*>(scl_v + step % 3 * SK + kg * TPW * kTileKeys + st * 16 + 4 * j);
+        vm = px_max3(px_max3(vm, vs[0], vs[1]), vs[2], vs[3]);
+      }
+      rn = fmaxf(r, __uint_as_float(__float_as_uint(px_col_max(vm)) & 0x7f800000u));
+    }
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {   // rare once a row has seen some keys
+    bool grow = KV8 && rn > r;
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) grow |= mn[cg] > m[cg];
+    if (__any(grow)) {
+      const float beta = KV8 ? r / rn : 1.f;
+      r = rn;
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) {
+        const float alpha = mn[cg] == m[cg] ? 1.f : __builtin_amdgcn_exp2f((m[cg] - mn[cg]) * c2);
+        m[cg] = mn[cg];
+        l[cg] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][cg] *= alpha * beta;
+      }
+    }
+  };
+  h8_t pb[TPW][CG];
+  auto probs = [&](const S_t& s, int step) __attribute__((always_inline)) {   // P^T and the row sums
+    const float ri = KV8 ? 1.f / r : 1.f;
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      const float mm = m[cg] == -INFINITY ? 0.f : m[cg] * c2;   // no valid key yet: masked scores give exp2(-inf) = 0
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        f4_t vs = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (KV8) vs = *reinterpret_cast<const f4_t*>(scl_v + step % 3 * SK + kg * TPW * kTileKeys + st * 16 + 4 * j) * ri;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[st][cg][i], c2, -mm));
+          l[cg] += p;
+          // fp16 (half a step: 2^-11 of the weight): the matrix units are what many rows wait for
+          pb[st / 2][cg][(st & 1) * 4 + i] = (_Float16)(KV8 ? p * vs[i] : p);
+        }
+      }
+    }
+  };
+  auto pv = [&](int step) __attribute__((always_inline)) {
+    const _Float16* vt = smem + (step % NS) * P::STAGE + (TPS + kg * TPW) * TILE;
+#pragma unroll
+    for (int tw = 0; tw < TPW; ++tw)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const h8_t va = *reinterpret_cast<const h8_t*>(vt + tw * TILE + (dt * 64 + lane) * 8);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) o[dt][cg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[tw][cg], o[dt][cg], 0, 0, 0);
+      }
+  };
+
+  // Software pipeline: step n forms P(n) from S(n) while the matrix cores take
+  // S(n + 1), then takes P(n) V(n) while the maximum of S(n + 1) is formed; it reads
+  // group n (K(n + 1), V(n)) from LDS.
+  S_t sa, sb;
+  __syncthreads();   // the piece before has left LDS
+  const uint32_t bad0 = bad & BITS;
+  id_k = fetch(1);
+  id_n = fetch(2);
+  if constexpr (KV8) {
+    load(pk, id_v, 0, 0, bad0);
+    store(pk, 0, 0, 0);
+    request(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+  } else {
+    dma(id_v, 0, 0);
+#pragma unroll
+    for (int g = 0; g < NS - 1; ++g) request(g);
+    wait_vm<(NS - 1) * 2 * PW>();
+  }
+  lds_barrier();
+  auto first = [&]() __attribute__((always_inline)) {
+    qk(sa, 0);
+    scale_mask(sa, 0, bad0);
+    row_max(sa, 0);
+    rescale();
+    arrive(0);
+  };
+  auto step = [&](S_t& cur, S_t& nxt, int n) __attribute__((always_inline)) {
+    request(n + NS - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    qk(nxt, n + 1);
+    probs(cur, n);
+    // P(n) is formed here, among the matrix instructions of S(n + 1), not moved down to its use
+#pragma unroll
+    for (int tw = 0; tw < TPW; ++tw)
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) asm volatile("" : "+v"(pb[tw][cg]));
+    __builtin_amdgcn_sched_barrier(0);
+    scale_mask(nxt, n + 1, bad >> (NS + 1) * TPS & BITS);   // fetched: up to step n + NS + 2
+    pv(n);
+    row_max(nxt, n + 1);
+    rescale();
+    arrive(n + 1);
+  };
+  if (idle) {   // the same requests and barriers
+    arrive(0);
+    for (int n = 0; n + 1 < n_steps; ++n) {
+      request(n + NS - 1);
+      arrive(n + 1);
+    }
+  } else {
+    first();
+    int n = 0;
+    for (; n + 2 < n_steps; n += 2) {
+      step(sa, sb, n);
+      step(sb, sa, n + 1);
+    }
+    if (n + 1 < n_steps) {
+      step(sa, sb, n);
+      probs(sb, n + 1);
+      pv(n + 1);
+    } else {
+      probs(sa, n);
+      pv(n);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the requests past the range land before the slots are reused
+  __syncthreads();
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    m[cg] *= c2;   // log2 units from here on
+    l[cg] += __shfl_xor(l[cg], 16, kWave);
+    l[cg] += __shfl_xor(l[cg], 32, kWave);
+    if constexpr (KV8) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt][cg] *= r;
+    }
+  }
+  if constexpr (KH > 1) {
+    // the other key groups' states into group 0's
+    f4_t* mg = reinterpret_cast<f4_t*>(smem);
+    if (kg > 0 && !idle) {
+      f4_t* w = mg + ((kg - 1) * RG + rg) * kWave * (P::STATE / 4) + lane;
+      *w = f4_t{m[0], l[0], m[1], l[1]};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) *(w += kWave) = o[dt][cg];
+    }
+    __syncthreads();
+    if (kg == 0 && !idle) {
+#pragma unroll
+      for (int k = 1; k < KH; ++k) {
+        const f4_t* w = mg + ((k - 1) * RG + rg) * kWave * (P::STATE / 4) + lane;
+        const f4_t ml = *w;
+        float f0[CG], f1[CG];
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+          const float m1 = ml[2 * cg], M = fmaxf(m[cg], m1);
+          f0[cg] = m[cg] == M ? 1.f : __builtin_amdgcn_exp2f(m[cg] - M);
+          f1[cg] = m1 == M ? 1.f : __builtin_amdgcn_exp2f(m1 - M);
+          m[cg] = M;
+          l[cg] = l[cg] * f0[cg] + ml[2 * cg + 1] * f1[cg];
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) {
+            const f4_t p = *(w += kWave);
+            o[dt][cg] = o[dt][cg] * f0[cg] + p * f1[cg];
+          }
+      }
+    }
+  }
+  if (kg == 0) {
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      const int row = rg * 32 + cg * 16 + h;
+      if (r0 + row >= R) continue;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4_t*>(o_out + (int64_t)row * HD + dt * 16 + 4 * j) = o[dt][cg];
+      if (j == 0) {
+        ml_out[2 * row] = m[cg];
+        ml_out[2 * row + 1] = l[cg];
+      }
+    }
+  }
+}
+
+template <int HD, int F, int ROWS>
+__global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
+  using P = PxForm<HD, F, ROWS>;
+  __shared__ __align__(16) _Float16 smem[P::SM];
+  __shared__ __align__(16) float scl[P::SCL];
   __shared__ int64_t cum[kPxMaxBatch + 1];
   __shared__ int64_t part[kPxWaves];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -282,22 +794,22 @@ __global__ __launch_bounds__(kPxThreads) void px_stage1(const PxArgs a) {
     for (int b = threadIdx.x; b <= a.batch; b += kPxThreads) a.plan[b] = cum[b];
     if (threadIdx.x == 0) a.plan[a.batch + 1] = ptiles;
   }
-  const int w = blockIdx.x * kPxWaves + wave;
   {
-    const int R = a.batch * a.g, n_rg = (R + 15) / 16;
-    const int64_t F_ = (int64_t)a.n_kv * n_rg * ptiles;
+    const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, steps = (ptiles + P::TPS - 1) / P::TPS, w = blockIdx.x;
     int64_t at, end;
-    share_of(w, F_, kPxListWaves, &at, &end);
+    share_of(w, (int64_t)a.n_kv * n_rb * steps, kPxBlocks, &at, &end);
     while (at < end) {
-      const int item = (int)(at / ptiles), ta = (int)(at - (int64_t)item * ptiles), kvh = item / n_rg, rg = item % n_rg;
-      const int tb = (int)min((int64_t)ptiles, ta + (end - at));
-      const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table};
-      px_piece<HD, F>(a, kv, kvh, rg * 16, min(16, R - rg * 16), 0, lp, ta, tb, a.pre_o + (int64_t)(w + item) * 16 * HD,
-                      a.pre_ml + (int64_t)(w + item) * 32, lane);
-      at += tb - ta;
+      const int item = (int)(at / steps), sa = (int)(at - (int64_t)item * steps), kvh = item / n_rb, rb = item % n_rb;
+      const int sb = (int)min((int64_t)steps, sa + (end - at));
+      float *o = a.pre_o + (int64_t)(w + item) * ROWS * HD, *ml = a.pre_ml + (int64_t)(w + item) * ROWS * 2;
+      const int tb = sa * P::TPS, te = min(sb * P::TPS, ptiles);
+      if constexpr (P::LDS) px_shared_piece<HD, F, ROWS>(a, smem, scl, kvh, rb * ROWS, R, lp, tb, te, o, ml);
+      else px_stream_piece<HD, F, ROWS>(a, reinterpret_cast<float*>(smem), kvh, rb * ROWS, R, lp, tb, te, o, ml);
+      at += sb - sa;
     }
   }
   {
+    const int w = blockIdx.x * kPxWaves + wave;
     const int64_t F_ = cum[a.batch] * a.n_kv;
     int64_t at, end;
     share_of(w, F_, kPxListWaves, &at, &end);
@@ -314,8 +826,8 @@ __global__ __launch_bounds__(kPxThreads) void px_stage1(const PxArgs a) {
       const int tb = (int)min((int64_t)nt, ta + (end - at));
       const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = lo >> 5;
       const PxKV kv{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages};
-      px_piece<HD, F>(a, kv, kvh, b * a.g, a.g, lo, hi, t0 + ta, t0 + tb, a.own_o + (int64_t)(w + item) * 16 * HD,
-                      a.own_ml + (int64_t)(w + item) * 32, lane);
+      px_own_piece<HD, F>(a, kv, kvh, b, lo, hi, t0 + ta, t0 + tb, a.own_o + (int64_t)(w + item) * 16 * HD,
+                          a.own_ml + (int64_t)(w + item) * 32, lane);
       at += tb - ta;
     }
   }
@@ -325,23 +837,23 @@ __global__ __launch_bounds__(kPxThreads) void px_stage1(const PxArgs a) {
 constexpr int kPxMergeThreads = 256;
 
 template <int HD>
-__global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a) {
+__global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a, int rows, int tps) {
   constexpr int TP = HD / 4, G = kPxMergeThreads / TP;   // threads of a piece, pieces at a time
   __shared__ f4_t so[G][TP];
   __shared__ float sm[G], sl[G];
   const int b = blockIdx.x / (a.n_kv * a.g), head = blockIdx.x % (a.n_kv * a.g), kvh = head / a.g, hh = head - kvh * a.g;
   if ((int)load_ctl_u32(a.len + b) < 0) return;
-  const int R = a.batch * a.g, n_rg = (R + 15) / 16, row = b * a.g + hh;
-  const int64_t ptiles = a.plan[a.batch + 1], c0 = a.plan[b], c1 = a.plan[b + 1], all = a.plan[a.batch] * a.n_kv;
+  const int n_rb = (a.batch * a.g + rows - 1) / rows, row = b * a.g + hh;
+  const int64_t steps = (a.plan[a.batch + 1] + tps - 1) / tps, c0 = a.plan[b], c1 = a.plan[b + 1], all = a.plan[a.batch] * a.n_kv;
   int n_pre = 0, n_own = 0;
   const float *po = nullptr, *pml = nullptr, *oo = nullptr, *oml = nullptr;
-  if (ptiles > 0) {
-    const int item = kvh * n_rg + row / 16;
-    const int64_t F = a.n_kv * n_rg * ptiles, x0 = item * ptiles;
-    const int w0 = worker_of(x0, F, kPxListWaves);
-    n_pre = worker_of(x0 + ptiles - 1, F, kPxListWaves) - w0 + 1;
-    po = a.pre_o + ((int64_t)(w0 + item) * 16 + row % 16) * HD;
-    pml = a.pre_ml + ((int64_t)(w0 + item) * 16 + row % 16) * 2;
+  if (steps > 0) {
+    const int item = kvh * n_rb + row / rows;
+    const int64_t F = a.n_kv * n_rb * steps, x0 = item * steps;
+    const int w0 = worker_of(x0, F, kPxBlocks);
+    n_pre = worker_of(x0 + steps - 1, F, kPxBlocks) - w0 + 1;
+    po = a.pre_o + ((int64_t)(w0 + item) * rows + row % rows) * HD;
+    pml = a.pre_ml + ((int64_t)(w0 + item) * rows + row % rows) * 2;
   }
   if (c1 > c0) {
     const int item = b * a.n_kv + kvh;
@@ -355,8 +867,8 @@ __global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a) {
   float M = -INFINITY, L = 0.f;
   f4_t O = {0.f, 0.f, 0.f, 0.f};
   for (int p = gi; p < n; p += G) {
-    const float* ml = p < n_pre ? pml + (int64_t)p * 32 : oml + (int64_t)(p - n_pre) * 32;
-    const float* op = p < n_pre ? po + (int64_t)p * 16 * HD : oo + (int64_t)(p - n_pre) * 16 * HD;
+    const float* ml = p < n_pre ? pml + (int64_t)p * rows * 2 : oml + (int64_t)(p - n_pre) * 32;
+    const float* op = p < n_pre ? po + (int64_t)p * rows * HD : oo + (int64_t)(p - n_pre) * 16 * HD;
     const float m1 = ml[0], l1 = ml[1];
     const f4_t o1 = *reinterpret_cast<const f4_t*>(op + 4 * d4);
     const float Mn = fmaxf(M, m1);
@@ -387,19 +899,22 @@ __global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a) {
   *reinterpret_cast<h4_t*>(a.out + b * a.out_stride + head * HD + 4 * d4) = v;
 }
 
+// Query rows of a block for R rows per kv head.
+int px_rows(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
+
 // Workspace: plan, then (m, l) and O of the own pieces and of the prefix's.
 struct PxSpace { size_t plan, own_ml, own_o, pre_ml, pre_o, bytes; };
 PxSpace px_space(int batch, int n_heads, int n_kv, int hd) {
-  const size_t g = n_heads / n_kv, n_rg = (batch * g + 15) / 16;
-  const size_t own = kPxListWaves + (size_t)batch * n_kv, pre = kPxListWaves + n_kv * n_rg;
+  const size_t R = (size_t)batch * (n_heads / n_kv), rows = px_rows(R);
+  const size_t own = kPxListWaves + (size_t)batch * n_kv, pre = (kPxBlocks + n_kv * ((R + rows - 1) / rows)) * rows;
   size_t off = 0;
   auto take = [&](size_t n) { const size_t o = off; off += (n + 255) & ~(size_t)255; return o; };
   PxSpace s;
   s.plan = take((batch + 2) * sizeof(int64_t));
   s.own_ml = take(own * 32 * 4);
   s.own_o = take(own * 16 * hd * 4);
-  s.pre_ml = take(pre * 32 * 4);
-  s.pre_o = take(pre * 16 * hd * 4);
+  s.pre_ml = take(pre * 2 * 4);
+  s.pre_o = take(pre * hd * 4);
   s.bytes = off;
   return s;
 }
@@ -409,10 +924,21 @@ bool px_shape_ok(int batch, int n_heads, int n_kv, int hd) {
          n_heads / n_kv <= 16 && (hd == 64 || hd == 128);
 }
 
+template <int HD, int F, int ROWS>
+void px_launch_rows(const PxArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((px_stage1<HD, F, ROWS>), dim3(kPxBlocks), dim3(kPxThreads), 0, st, a);
+  hipLaunchKernelGGL((px_merge<HD>), dim3(a.batch * a.n_kv * a.g), dim3(kPxMergeThreads), 0, st, a, ROWS, PxForm<HD, F, ROWS>::TPS);
+}
+
 template <int HD, int F>
 void px_launch(const PxArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((px_stage1<HD, F>), dim3(kPxBlocks), dim3(kPxThreads), 0, st, a);
-  hipLaunchKernelGGL((px_merge<HD>), dim3(a.batch * a.n_kv * a.g), dim3(kPxMergeThreads), 0, st, a);
+  switch (px_rows((int64_t)a.batch * a.g)) {
+    case 16: px_launch_rows<HD, F, 16>(a, st); break;
+    case 32: px_launch_rows<HD, F, 32>(a, st); break;
+    case 64: px_launch_rows<HD, F, 64>(a, st); break;
+    case 128: px_launch_rows<HD, F, 128>(a, st); break;
+    default: px_launch_rows<HD, F, 256>(a, st);
+  }
 }
 
 template <int HD>
