@@ -283,13 +283,13 @@ __device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, in
   }
 }
 
-// How a block attends over the prefix with ROWS query rows.  Up to 32 rows every wave
+// How a block attends over the prefix with ROWS query rows.  Up to 64 rows every wave
 // takes 16 of them over tiles of its own in registers (the K / V operands feed one
 // instruction each, and HBM is what bounds it); beyond that 32 rows over tiles in LDS,
 // which the row groups share.  KH waves share a row group's keys.
 template <int HD, int F, int ROWS>
 struct PxForm {
-  static constexpr bool LDS = ROWS > 32;
+  static constexpr bool LDS = ROWS > 64;
   static constexpr int WR = LDS ? 32 : 16;              // rows of a wave
   static constexpr int RG = ROWS / WR, KH = kPxWaves / RG;
   static constexpr int TPW = !LDS ? 1 : KH == 1 ? 2 : KH == 2 ? (HD == 128 && F != CQ_KV_FP16 ? 1 : 2) : (HD == 64 ? 2 : 1);
@@ -305,7 +305,7 @@ struct PxForm {
   static constexpr int SCL = LDS && F != CQ_KV_FP16 ? (NS + 3) * TPS * kTileKeys : 1;   // K scales per slot, V scales three steps
 };
 
-// Tiles [tb, te) of the prefix for up to 32 rows.
+// Tiles [tb, te) of the prefix for up to 64 rows.
 template <int HD, int F, int ROWS>
 __device__ __forceinline__ void px_stream_piece(const PxArgs& a, float* sm, int kvh, int r0, int R, int lp, int tb, int te, float* o,
                                                 float* ml) {
@@ -351,7 +351,7 @@ __device__ __forceinline__ void px_stream_piece(const PxArgs& a, float* sm, int 
   }
 }
 
-// Tiles [tb, te) of the prefix for 64, 128 or 256 rows: the prefill attention's loop
+// Tiles [tb, te) of the prefix for 128 or 256 rows: the prefill attention's loop
 // over pages, without its causal limits.
 template <int HD, int F, int ROWS>
 __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem, float* scl, int kvh, int r0, int R, int lp, int tb, int te,
@@ -833,18 +833,24 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   }
 }
 
-// Joins the pieces of one row (b, head): a block of HD / 4 threads per piece group.
+// Joins the pieces of one row (b, head), a block per row: the pieces' (m, l), one per
+// thread, give each piece's weight 2^(m - M) and the row's sum; then G groups of HD / 4
+// threads add up the weighted O, kAhead pieces of each group requested before the
+// weights are known.  What bounds it: three memory round trips (lengths, first pieces,
+// rest), and HBM for many rows of many pieces.
 constexpr int kPxMergeThreads = 256;
 
 template <int HD>
 __global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a, int rows, int tps) {
   constexpr int TP = HD / 4, G = kPxMergeThreads / TP;   // threads of a piece, pieces at a time
+  constexpr int kAhead = 4, W = kPxMergeThreads / kWave;
   __shared__ f4_t so[G][TP];
-  __shared__ float sm[G], sl[G];
+  __shared__ float weight[kPxMergeThreads], red[2][W];
   const int b = blockIdx.x / (a.n_kv * a.g), head = blockIdx.x % (a.n_kv * a.g), kvh = head / a.g, hh = head - kvh * a.g;
-  if ((int)load_ctl_u32(a.len + b) < 0) return;
   const int n_rb = (a.batch * a.g + rows - 1) / rows, row = b * a.g + hh;
+  const int len = (int)load_ctl_u32(a.len + b);
   const int64_t steps = (a.plan[a.batch + 1] + tps - 1) / tps, c0 = a.plan[b], c1 = a.plan[b + 1], all = a.plan[a.batch] * a.n_kv;
+  if (len < 0) return;
   int n_pre = 0, n_own = 0;
   const float *po = nullptr, *pml = nullptr, *oo = nullptr, *oml = nullptr;
   if (steps > 0) {
@@ -863,35 +869,53 @@ __global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a, int 
     oo = a.own_o + ((int64_t)(w0 + item) * 16 + hh) * HD;
     oml = a.own_ml + ((int64_t)(w0 + item) * 16 + hh) * 2;
   }
-  const int gi = threadIdx.x / TP, d4 = threadIdx.x % TP, n = n_pre + n_own;
+  const int tid = threadIdx.x, gi = tid / TP, d4 = tid % TP, lane = tid & (kWave - 1), n = n_pre + n_own;
+  auto ml_of = [&](int p) { return p < n_pre ? pml + (int64_t)p * rows * 2 : oml + (int64_t)(p - n_pre) * 32; };
+  auto o_of = [&](int p) {
+    return *reinterpret_cast<const f4_t*>((p < n_pre ? po + (int64_t)p * rows * HD : oo + (int64_t)(p - n_pre) * 16 * HD) + 4 * d4);
+  };
   float M = -INFINITY, L = 0.f;
   f4_t O = {0.f, 0.f, 0.f, 0.f};
-  for (int p = gi; p < n; p += G) {
-    const float* ml = p < n_pre ? pml + (int64_t)p * rows * 2 : oml + (int64_t)(p - n_pre) * 32;
-    const float* op = p < n_pre ? po + (int64_t)p * rows * HD : oo + (int64_t)(p - n_pre) * 16 * HD;
-    const float m1 = ml[0], l1 = ml[1];
-    const f4_t o1 = *reinterpret_cast<const f4_t*>(op + 4 * d4);
-    const float Mn = fmaxf(M, m1);
-    const float f0 = M == Mn ? 1.f : __builtin_amdgcn_exp2f(M - Mn), f1 = m1 == Mn ? 1.f : __builtin_amdgcn_exp2f(m1 - Mn);
+  for (int p0 = 0; p0 < n; p0 += kPxMergeThreads) {
+    const int here = min(n - p0, kPxMergeThreads);
+    float m1 = -INFINITY, l1 = 0.f;
+    if (tid < here) {
+      const float* ml = ml_of(p0 + tid);
+      m1 = ml[0];
+      l1 = ml[1];
+    }
+    f4_t first[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) first[i] = i * G + gi < here ? o_of(p0 + i * G + gi) : f4_t{0.f, 0.f, 0.f, 0.f};
+    const float mw = wave_max(m1);
+    if (p0 > 0) __syncthreads();   // the weights before have been read
+    if (lane == 0) red[0][tid / kWave] = mw;
+    __syncthreads();
+    float Mn = M;
+#pragma unroll
+    for (int w = 0; w < W; ++w) Mn = fmaxf(Mn, red[0][w]);
+    // a row that has seen nothing: m = M = -inf, with l and O of zero
+    const float f = m1 == Mn ? 1.f : __builtin_amdgcn_exp2f(m1 - Mn), f0 = M == Mn ? 1.f : __builtin_amdgcn_exp2f(M - Mn);
+    weight[tid] = f;
+    const float lw = wave_sum(l1 * f);
+    if (lane == 0) red[1][tid / kWave] = lw;
+    __syncthreads();
     M = Mn;
-    L = L * f0 + l1 * f1;
-    O = O * f0 + o1 * f1;
+    L *= f0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) L += red[1][w];
+    O *= f0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i * G + gi < here) O += first[i] * weight[i * G + gi];
+#pragma unroll 4
+    for (int p = kAhead * G + gi; p < here; p += G) O += o_of(p0 + p) * weight[p];
   }
-  if (d4 == 0) { sm[gi] = M; sl[gi] = L; }
   so[gi][d4] = O;
   __syncthreads();
   if (gi != 0) return;
-  M = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < G; ++k) M = fmaxf(M, sm[k]);
-  L = 0.f;
-  O = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < G; ++k) {
-    const float f = sm[k] == M ? 1.f : __builtin_amdgcn_exp2f(sm[k] - M);
-    L += sl[k] * f;
-    O += so[k][d4] * f;
-  }
+  for (int k = 1; k < G; ++k) O += so[k][d4];
   const float inv = L == 0.f ? 0.f : 1.f / L;
   h4_t v;
 #pragma unroll
