@@ -3,18 +3,25 @@
 // each sequence's own pages for its own rows.  No counterpart in the reference.
 //
 // For row (b, head h of kv head kvh): s_t = q . k_t / sqrt(hd) over the prefix's and
-// the sequence's own positions, out = sum exp(s_t - m) v_t / sum exp(s_t - m), formed
-// in pieces: each piece of keys leaves (m, l, O) in fp32, and a second launch joins the
-// pieces of a row by the log-sum-exp rule.
+// the sequence's own positions, out = sum exp(s_t - m) v_t / sum exp(s_t - m).  Two
+// launches:
+//   * px_stage1: the prefix, for all rows of a kv head together, in pieces of keys that
+//     leave (m, l, O) in fp32; and of very long sequences the own tiles past the first
+//     few;
+//   * px_finish: a block per (sequence, kv head) attends over the sequence's own tiles,
+//     joins the pieces of its rows by the log-sum-exp rule and writes the output.
+// Where the tables are short px_finish takes the prefix too, once for each sequence, and
+// is the only launch; where only the lengths are short (known on the device alone) it
+// does so behind a first launch with nothing to do.
 //
 // Work of stage 1, whose grid is one block per CU: the steps (a few 32-key tiles) of
 // all items of the prefix, an item being (kv head, block of query rows), form one
-// list that the blocks share evenly, and the tiles of all (sequence, kv head) items
-// of the own part one that the waves share evenly (share_of), wherever item borders
+// list that its blocks share evenly, and the far tiles of all (sequence, kv head) items
+// one that the waves of the other blocks share evenly (share_of), wherever item borders
 // fall, from the lengths found on the device: lengths may be ragged, and a captured
 // launch serves other lengths.  Worker w's piece of item i is stored in slot w + i
-// (either w or i grows from one piece to the next, so slots differ), and the joining
-// launch finds a row's pieces by the same arithmetic.
+// (either w or i grows from one piece to the next, so slots differ), and px_finish
+// finds a row's pieces by the same arithmetic.
 #include "cq_attention.h"
 #include "cq_pages.h"
 
@@ -27,7 +34,7 @@ namespace {
 
 constexpr int kPxWaves = 8, kPxThreads = kPxWaves * kWave;
 constexpr int kPxBlocks = kNumCUs;                    // one block per CU
-constexpr int kPxListWaves = kPxBlocks * kPxWaves;    // workers of the own list
+constexpr int kPxListWaves = kPxBlocks * kPxWaves;    // most workers of the far own tiles
 constexpr int kPxMaxBatch = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -45,21 +52,27 @@ struct PxArgs {
   int pre_pages, max_pages;
   int batch, n_kv, g;
   // workspace
-  int64_t* plan;                  // [batch + 1] own tiles before each sequence, then the prefix's tiles
+  int64_t* plan;                  // [batch + 1] own tiles before each sequence, then the prefix's steps and blocks
   float* own_o;                   // [slot][16][HD]
   float* own_ml;                  // [slot][16][2]
   float* pre_o;                   // [slot][rows of a block][HD]
   float* pre_ml;
 };
 
+// a / b for a >= 0, b > 0; in 32 bits where they do (64-bit divisions are a microsecond of
+// code each, and lists of so many tiles are rare).
+__device__ __forceinline__ int64_t px_div(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 // Range [first, end) of worker w when F tiles are shared by W workers (the first F
 // workers, a tile each, if there are fewer tiles): F w / W, F (w + 1) / W.
 __device__ __forceinline__ void share_of(int w, int64_t F, int W, int64_t* first, int64_t* end) {
-  *first = F <= W ? min((int64_t)w, F) : F * w / W;
-  *end = F <= W ? min((int64_t)w + 1, F) : F * (w + 1) / W;
+  *first = F <= W ? min((int64_t)w, F) : px_div(F * w, W);
+  *end = F <= W ? min((int64_t)w + 1, F) : px_div(F * (w + 1), W);
 }
 // The worker that has tile x.
-__device__ __forceinline__ int worker_of(int64_t x, int64_t F, int W) { return (int)(F <= W ? x : ((x + 1) * W - 1) / F); }
+__device__ __forceinline__ int worker_of(int64_t x, int64_t F, int W) { return (int)(F <= W ? x : px_div((x + 1) * W - 1, F)); }
 
 // Largest of v over the four lanes that share a column (lane % 16).  The two results
 // of a swap go through variables: a bit cast of an element of the builtin's vector
@@ -76,16 +89,29 @@ __device__ __forceinline__ float px_col_max(float v) {
 // One v_max3_f32 (left to the compiler, which knows the wait states of matrix results).
 __device__ __forceinline__ float px_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
+// Own tiles of a sequence that px_finish takes; stage 1 takes those behind them.  With
+// few blocks in the second launch the first one's others are there for them.
+__device__ __forceinline__ int px_near(const PxArgs& a) { return a.batch * a.n_kv <= 64 ? 16 : 64; }
+
+// Whether px_finish takes the prefix: `ptiles` tiles for each of its blocks, against a
+// first launch whose pieces have a chain of their own (some 10 us).  Measured, 7B heads,
+// fp16: 8 sequences over 1500 tokens 11.6 us so and 13.4 in pieces, over 2500 17.4 and
+// 14.5; 64 over 2000 18.0 and 28.5.
+__device__ __host__ __forceinline__ bool px_prefix_near(int batch, int n_kv, int64_t ptiles) {
+  return ptiles * std::max(190, batch * n_kv) <= 190 * 56;
+}
+
 // Positions that a table of n pages holds, and the length cut there.
 __device__ __forceinline__ int cut_len(int len, int pages, int shift) {
   return min(max(len, 0), (int)min((int64_t)pages << shift, (int64_t)0x7fffffff));
 }
 
-// One kv head of a paged cache as a wave's tiles see it.
+// Positions [lo, hi) of one kv head of a paged cache.
 struct PxKV {
   PageView pv;
   int64_t off;       // elements: layer and head
   const int* table;  // page of each run of page_tokens positions
+  int lo, hi;
 };
 
 // The K and V of one 32-key tile in matrix operand order, and where its keys are valid.
@@ -96,10 +122,10 @@ struct PxTile {
   int lo, hi;        // valid keys of the tile: [lo, hi)
 };
 
-// Requests tile ti (positions [32 ti, 32 ti + 32) cut to [lo, hi)); with `want` false,
+// Requests tile ti (positions [32 ti, 32 ti + 32) cut to kv's); with `want` false,
 // or a page outside the pool, nothing is read and no key is valid.
 template <int HD, int F>
-__device__ __forceinline__ void px_load(PxTile<HD, F>& t, const PxKV& kv, int ti, int lo, int hi, bool want, int lane) {
+__device__ __forceinline__ void px_load(PxTile<HD, F>& t, const PxKV& kv, int ti, bool want, int lane) {
   constexpr int ES = F == CQ_KV_FP16 ? 2 : 1, N = F == CQ_KV_FP16 ? HD / 16 : HD / 32;
   const int s5 = kv.pv.shift - 5;
   int page = want ? (int)load_ctl_u32(kv.table + (ti >> s5)) : -1;
@@ -123,8 +149,8 @@ __device__ __forceinline__ void px_load(PxTile<HD, F>& t, const PxKV& kv, int ti
       t.vs[st] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rvs, (st * 16 + 4 * j) * 4, 0, 0));
     }
   }
-  t.lo = ok ? lo - 32 * ti : 0;
-  t.hi = ok ? hi - 32 * ti : 0;
+  t.lo = ok ? kv.lo - 32 * ti : 0;
+  t.hi = ok ? kv.hi - 32 * ti : 0;
 }
 
 // Operand i of a tile's K (or V) as fp16.
@@ -229,17 +255,18 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
   }
 }
 
-// Tiles ta, ta + step, ... < tb of one cache for the rows q[r0 .. r0 + rows) of a kv
-// head: the wave's state, m in log2 units and O in the values' own units.
-template <int HD, int F>
-__device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, const PxKV& kv, int kvh, int r0, int rows, int lo, int hi, int ta,
-                                       int tb, int step, int lane) {
+// Tiles ta, ta + step, ... < tb for the rows q[r0 .. r0 + rows) of a kv head: the
+// wave's state, m in log2 units and O in the values' own units.  load(tile, k) requests
+// tile k.
+template <int HD, int F, class Load>
+__device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, int kvh, int r0, int rows, int ta, int tb, int step, int lane,
+                                       Load load) {
   constexpr int KK = HD / 32, DT = HD / 16;
   const int h = lane & 15, j = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);
   const uint32_t magic = vgpr_const(0x64646464u);
   PxTile<HD, F> A, B;
-  px_load<HD, F>(A, kv, ta, lo, hi, ta < tb, lane);
+  load(A, ta);
   h8_t qb[KK];
   const int r = r0 + min(h, rows - 1), b = r / a.g;
   const _Float16* q = a.q + b * a.q_stride + (kvh * a.g + (r - b * a.g)) * HD;
@@ -251,10 +278,10 @@ __device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, const P
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) st.o[dt] = f4_t{0.f, 0.f, 0.f, 0.f};
   for (int ti = ta; ti < tb; ti += 2 * step) {
-    px_load<HD, F>(B, kv, ti + step, lo, hi, ti + step < tb, lane);
+    load(B, ti + step);
     px_attend<HD, F>(A, qb, st, c2, lane, magic);
     if (ti + step >= tb) break;
-    px_load<HD, F>(A, kv, ti + 2 * step, lo, hi, ti + 2 * step < tb, lane);
+    load(A, ti + 2 * step);
     px_attend<HD, F>(B, qb, st, c2, lane, magic);
   }
   st.m *= c2;
@@ -266,13 +293,13 @@ __device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, const P
   }
 }
 
-// The own part's piece: one wave's.
+// A piece of the own part: one wave's.
 template <int HD, int F>
-__device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, int kvh, int b, int lo, int hi, int ta, int tb, float* o,
-                                             float* ml, int lane) {
+__device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, int kvh, int b, int ta, int tb, float* o, float* ml, int lane) {
   const int h = lane & 15, j = lane >> 4;
   PxState<HD> st;
-  px_run<HD, F>(st, a, kv, kvh, b * a.g, a.g, lo, hi, ta, tb, 1, lane);
+  px_run<HD, F>(st, a, kvh, b * a.g, a.g, ta, tb, 1, lane,
+                [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) { px_load<HD, F>(t, kv, k, k < tb, lane); });
   if (h < a.g) {
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) *reinterpret_cast<f4_t*>(o + h * HD + dt * 16 + 4 * j) = st.o[dt];
@@ -282,6 +309,51 @@ __device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, in
     }
   }
 }
+
+// Joins the states of the waves k * RG + rg, k < KH, through LDS (sm: W (2 + DT * 16)
+// * 16 floats for W waves): every wave of the block calls it, and gets in O the dim
+// tiles kg, kg + KH, ... of its row group, in M and L the joined statistics.
+template <int HD, int RG, int KH>
+struct PxJoin {
+  static constexpr int DT = HD / 16, PER = (DT + KH - 1) / KH;
+  float M, L;
+  f4_t O[PER];
+  __device__ __forceinline__ void run(const PxState<HD>& st, float* sm, int wave, int lane) {
+    float* ml = sm + RG * KH * DT * kWave * 4;   // [wave][16][2]
+    f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * DT * kWave + lane;
+    const int rg = wave % RG, kg = wave / RG, h = lane & 15;
+    __syncthreads();   // LDS may be in use
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) w[dt * kWave] = st.o[dt];
+    if (lane < 16) {
+      ml[(wave * 16 + h) * 2] = st.m;
+      ml[(wave * 16 + h) * 2 + 1] = st.l;
+    }
+    __syncthreads();
+    float m1[KH];
+    M = -INFINITY;
+    L = 0.f;
+#pragma unroll
+    for (int k = 0; k < KH; ++k) {
+      m1[k] = ml[((k * RG + rg) * 16 + h) * 2];
+      M = fmaxf(M, m1[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < KH; ++k) {
+      m1[k] = m1[k] == M ? 1.f : __builtin_amdgcn_exp2f(m1[k] - M);
+      L += ml[((k * RG + rg) * 16 + h) * 2 + 1] * m1[k];
+    }
+    const f4_t* s = reinterpret_cast<const f4_t*>(sm) + lane;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      O[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+      if (kg + i * KH < DT) {
+#pragma unroll
+        for (int k = 0; k < KH; ++k) O[i] += s[((k * RG + rg) * DT + kg + i * KH) * kWave] * m1[k];
+      }
+    }
+  }
+};
 
 // How a block attends over the prefix with ROWS query rows.  Up to 64 rows every wave
 // takes 16 of them over tiles of its own in registers (the K / V operands feed one
@@ -299,9 +371,9 @@ struct PxForm {
   // LDS slots: three (requests two steps ahead) where they fit 96 KB, else two
   static constexpr int NS = F == CQ_KV_FP16 && 3 * STAGE * 2 <= 96 * 1024 ? 3 : 2;
   static constexpr int DT = HD / 16, CG = WR / 16;
-  static constexpr int STATE = 4 + 4 * DT * CG;         // floats of one lane's softmax state: (m, l) of up to two slices, O
+  static constexpr int STATE = 4 + 4 * DT * CG;         // floats of one lane's softmax state in LDS (two slices): (m, l) of each, O
   // halves of LDS: the stages, over them the states of the other key groups
-  static constexpr int SM = LDS ? std::max(NS * STAGE, (KH - 1) * RG * kWave * STATE * 2) : kPxWaves * kWave * STATE * 2;
+  static constexpr int SM = LDS ? std::max(NS * STAGE, (KH - 1) * RG * kWave * STATE * 2) : kPxWaves * 16 * (2 + HD) * 2;
   static constexpr int SCL = LDS && F != CQ_KV_FP16 ? (NS + 3) * TPS * kTileKeys : 1;   // K scales per slot, V scales three steps
 };
 
@@ -313,41 +385,21 @@ __device__ __forceinline__ void px_stream_piece(const PxArgs& a, float* sm, int 
   constexpr int DT = HD / 16, RG = P::RG, KH = P::KH;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rg = wave % RG, kg = wave / RG, rw = r0 + rg * 16;
-  const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table};
+  const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
   PxState<HD> st;
-  px_run<HD, F>(st, a, kv, kvh, min(rw, R - 1), max(min(16, R - rw), 1), 0, lp, tb + kg, rw < R ? te : tb, KH, lane);
-  // the key groups' states through LDS: [wave][1 + DT][lane] of (m, l, -, -), O
-  static_assert(P::STATE == 4 * (1 + DT), "LDS holds the states");
-  f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * (1 + DT) * kWave + lane;
-  __syncthreads();
-  *w = f4_t{st.m, st.l, 0.f, 0.f};
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) w[(1 + dt) * kWave] = st.o[dt];
-  __syncthreads();
-  // a wave joins DT / KH of its row group's dim tiles (KH = 8 with DT = 4: half of the waves)
+  const int end = rw < R ? te : tb;   // a wave without rows takes no tile
+  px_run<HD, F>(st, a, kvh, min(rw, R - 1), max(min(16, R - rw), 1), tb + kg, end, KH, lane,
+                [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) { px_load<HD, F>(t, kv, k, k < end, lane); });
+  PxJoin<HD, RG, KH> jn;
+  jn.run(st, sm, wave, lane);
   const int h = lane & 15, j = lane >> 4;
   if (rw + h >= R) return;
-  const f4_t* s = reinterpret_cast<const f4_t*>(sm) + lane;
-  float m1[KH], M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int k = 0; k < KH; ++k) {
-    m1[k] = s[(k * RG + rg) * (1 + DT) * kWave][0];
-    M = fmaxf(M, m1[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < KH; ++k) {
-    m1[k] = m1[k] == M ? 1.f : __builtin_amdgcn_exp2f(m1[k] - M);
-    L += s[(k * RG + rg) * (1 + DT) * kWave][1] * m1[k];
-  }
-  for (int dt = kg; dt < DT; dt += KH) {
-    f4_t O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < KH; ++k) O += s[((k * RG + rg) * (1 + DT) + 1 + dt) * kWave] * m1[k];
-    *reinterpret_cast<f4_t*>(o + (rg * 16 + h) * HD + dt * 16 + 4 * j) = O;
-  }
+  for (int i = 0; i < jn.PER; ++i)
+    if (kg + i * KH < DT) *reinterpret_cast<f4_t*>(o + (rg * 16 + h) * HD + (kg + i * KH) * 16 + 4 * j) = jn.O[i];
   if (kg == 0 && j == 0) {
-    ml[2 * (rg * 16 + h)] = M;
-    ml[2 * (rg * 16 + h) + 1] = L;
+    ml[2 * (rg * 16 + h)] = jn.M;
+    ml[2 * (rg * 16 + h) + 1] = jn.L;
   }
 }
 
@@ -759,6 +811,24 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   }
 }
 
+// Blocks that take the prefix, of kPxBlocks; the others take the own part.  Each kind
+// of work has a chain of its own from first load to stored piece (some 7 us), which a
+// block that does both would pay twice.  Costs in block time, microseconds: a step of
+// the prefix, an own tile, an own piece.
+template <int HD, int F, int ROWS>
+__device__ __forceinline__ int px_pre_blocks(int64_t pre_steps, int64_t pre_items, int64_t own_tiles, int64_t own_items) {
+  using P = PxForm<HD, F, ROWS>;
+  if (own_tiles == 0) return kPxBlocks;
+  if (pre_steps == 0) return 0;
+  constexpr float tile = HD == 128 ? 0.8f : 0.4f;
+  const float pre = (float)pre_steps * (P::TPS * tile * (ROWS <= 64 ? 1.f : ROWS == 128 ? 0.9f : 1.7f)) + (float)min(pre_items, pre_steps) * (P::LDS ? 7.f : 3.f);
+  const float own = (float)own_tiles * (tile * 0.8f) + (float)min(own_items, own_tiles) * 0.4f;
+  int n = (int)((float)kPxBlocks * pre / (pre + own) + 0.5f);
+  n = max(n, kPxBlocks - (int)min((own_tiles + kPxWaves - 1) / kPxWaves, (int64_t)kPxBlocks));   // no more blocks than tiles for their waves
+  n = min(n, (int)min(pre_steps, (int64_t)kPxBlocks));
+  return min(max(n, 1), kPxBlocks - 1);
+}
+
 template <int HD, int F, int ROWS>
 __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   using P = PxForm<HD, F, ROWS>;
@@ -769,12 +839,13 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lp = cut_len((int)load_ctl_u32(a.pre_len), a.pre_pages, a.pre.shift);
   const int lo = a.start ? max((int)load_ctl_u32(a.start), 0) : 0;
-  // own tiles before each sequence
+  // far own tiles before each sequence
+  const int near = px_near(a);
   int64_t n2[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int b = 2 * threadIdx.x + i, hi = b < a.batch ? cut_len(a.len[b], a.max_pages, a.own.shift) : 0;
-    n2[i] = hi > lo ? (int64_t)((hi - 1) >> 5) - (lo >> 5) + 1 : 0;
+    n2[i] = hi > lo ? max((int64_t)((hi - 1) >> 5) - (lo >> 5) + 1 - near, (int64_t)0) : 0;
   }
   int64_t x = n2[0] + n2[1];
 #pragma unroll
@@ -789,17 +860,22 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   cum[2 * threadIdx.x + 2] = x;
   if (threadIdx.x == 0) cum[0] = 0;
   __syncthreads();
-  const int ptiles = (lp + 31) >> 5;
+  const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, ptiles = (lp + 31) >> 5, steps = px_prefix_near(a.batch, a.n_kv, ptiles) ? 0 : (ptiles + P::TPS - 1) / P::TPS;
+  const int64_t pre_steps = (int64_t)a.n_kv * n_rb * steps, own_tiles = cum[a.batch] * a.n_kv;
+  const int n_pre = px_pre_blocks<HD, F, ROWS>(pre_steps, a.n_kv * n_rb, own_tiles, (int64_t)a.batch * a.n_kv);
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b <= a.batch; b += kPxThreads) a.plan[b] = cum[b];
-    if (threadIdx.x == 0) a.plan[a.batch + 1] = ptiles;
+    if (threadIdx.x == 0) {
+      a.plan[a.batch + 1] = steps;
+      a.plan[a.batch + 2] = n_pre;
+    }
   }
-  {
-    const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, steps = (ptiles + P::TPS - 1) / P::TPS, w = blockIdx.x;
-    int64_t at, end;
-    share_of(w, (int64_t)a.n_kv * n_rb * steps, kPxBlocks, &at, &end);
+  int64_t at, end;
+  if ((int)blockIdx.x < n_pre) {
+    const int w = blockIdx.x;
+    share_of(w, pre_steps, n_pre, &at, &end);
     while (at < end) {
-      const int item = (int)(at / steps), sa = (int)(at - (int64_t)item * steps), kvh = item / n_rb, rb = item % n_rb;
+      const int item = (int)px_div(at, steps), sa = (int)(at - (int64_t)item * steps), kvh = item / n_rb, rb = item % n_rb;
       const int sb = (int)min((int64_t)steps, sa + (end - at));
       float *o = a.pre_o + (int64_t)(w + item) * ROWS * HD, *ml = a.pre_ml + (int64_t)(w + item) * ROWS * 2;
       const int tb = sa * P::TPS, te = min(sb * P::TPS, ptiles);
@@ -807,120 +883,111 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
       else px_stream_piece<HD, F, ROWS>(a, reinterpret_cast<float*>(smem), kvh, rb * ROWS, R, lp, tb, te, o, ml);
       at += sb - sa;
     }
+    return;
   }
-  {
-    const int w = blockIdx.x * kPxWaves + wave;
-    const int64_t F_ = cum[a.batch] * a.n_kv;
-    int64_t at, end;
-    share_of(w, F_, kPxListWaves, &at, &end);
-    while (at < end) {
-      int b = 0, top = a.batch;   // last b with n_kv * cum[b] <= at
-      while (top - b > 1) {
-        const int mid = (b + top) / 2;
-        if (cum[mid] * a.n_kv <= at) b = mid; else top = mid;
-      }
-      b = __builtin_amdgcn_readfirstlane(b);
-      const int nt = (int)(cum[b + 1] - cum[b]);
-      const int64_t in = at - cum[b] * a.n_kv;
-      const int kvh = (int)(in / nt), ta = (int)(in - (int64_t)kvh * nt), item = b * a.n_kv + kvh;
-      const int tb = (int)min((int64_t)nt, ta + (end - at));
-      const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = lo >> 5;
-      const PxKV kv{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages};
-      px_own_piece<HD, F>(a, kv, kvh, b, lo, hi, t0 + ta, t0 + tb, a.own_o + (int64_t)(w + item) * 16 * HD,
-                          a.own_ml + (int64_t)(w + item) * 32, lane);
-      at += tb - ta;
+  const int w = (blockIdx.x - n_pre) * kPxWaves + wave;
+  share_of(w, own_tiles, (kPxBlocks - n_pre) * kPxWaves, &at, &end);
+  while (at < end) {
+    int b = 0, top = a.batch;   // last b with n_kv * cum[b] <= at
+    while (top - b > 1) {
+      const int mid = (b + top) / 2;
+      if (cum[mid] * a.n_kv <= at) b = mid; else top = mid;
     }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const int nt = (int)(cum[b + 1] - cum[b]);
+    const int64_t in = at - cum[b] * a.n_kv;
+    const int kvh = (int)px_div(in, nt), ta = (int)(in - (int64_t)kvh * nt), item = b * a.n_kv + kvh;
+    const int tb = (int)min((int64_t)nt, ta + (end - at));
+    const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = (lo >> 5) + near;
+    const PxKV kv{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
+    px_own_piece<HD, F>(a, kv, kvh, b, t0 + ta, t0 + tb, a.own_o + (int64_t)(w + item) * 16 * HD, a.own_ml + (int64_t)(w + item) * 32, lane);
+    at += tb - ta;
   }
 }
 
-// Joins the pieces of one row (b, head), a block per row: the pieces' (m, l), one per
-// thread, give each piece's weight 2^(m - M) and the row's sum; then G groups of HD / 4
-// threads add up the weighted O, kAhead pieces of each group requested before the
-// weights are known.  What bounds it: three memory round trips (lengths, first pieces,
-// rest), and HBM for many rows of many pieces.
-constexpr int kPxMergeThreads = 256;
-
+// A piece's state joined into a wave's (whose m is in log2 units, l complete in every
+// lane): o, ml point to the row of this lane.
 template <int HD>
-__global__ __launch_bounds__(kPxMergeThreads) void px_merge(const PxArgs a, int rows, int tps) {
-  constexpr int TP = HD / 4, G = kPxMergeThreads / TP;   // threads of a piece, pieces at a time
-  constexpr int kAhead = 4, W = kPxMergeThreads / kWave;
-  __shared__ f4_t so[G][TP];
-  __shared__ float weight[kPxMergeThreads], red[2][W];
-  const int b = blockIdx.x / (a.n_kv * a.g), head = blockIdx.x % (a.n_kv * a.g), kvh = head / a.g, hh = head - kvh * a.g;
-  const int n_rb = (a.batch * a.g + rows - 1) / rows, row = b * a.g + hh;
+__device__ __forceinline__ void px_absorb(PxState<HD>& st, const float* o, const float* ml, int j) {
+  constexpr int DT = HD / 16;
+  const float m1 = ml[0], l1 = ml[1];
+  f4_t v[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) v[dt] = *reinterpret_cast<const f4_t*>(o + dt * 16 + 4 * j);
+  const float M = fmaxf(st.m, m1);
+  const float f0 = st.m == M ? 1.f : __builtin_amdgcn_exp2f(st.m - M), f1 = m1 == M ? 1.f : __builtin_amdgcn_exp2f(m1 - M);
+  st.m = M;
+  st.l = st.l * f0 + l1 * f1;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) st.o[dt] = st.o[dt] * f0 + v[dt] * f1;
+}
+
+// Block (sequence b, kv head): the near own tiles (and a near prefix's), W waves taking
+// every W-th; then, with PIECES, the pieces that stage 1 left, every W-th too.  The
+// waves join in LDS.
+template <int HD, int F, int W, bool PIECES>
+__global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int rows) {
+  constexpr int DT = HD / 16;
+  __shared__ __align__(16) float sm[W * 16 * (2 + HD)];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int h = lane & 15, j = lane >> 4;
+  const int b = blockIdx.x / a.n_kv, kvh = blockIdx.x - b * a.n_kv;
   const int len = (int)load_ctl_u32(a.len + b);
-  const int64_t steps = (a.plan[a.batch + 1] + tps - 1) / tps, c0 = a.plan[b], c1 = a.plan[b + 1], all = a.plan[a.batch] * a.n_kv;
+  const int lp = cut_len((int)load_ctl_u32(a.pre_len), a.pre_pages, a.pre.shift);
+  const int lo = a.start ? max((int)load_ctl_u32(a.start), 0) : 0;
   if (len < 0) return;
-  int n_pre = 0, n_own = 0;
-  const float *po = nullptr, *pml = nullptr, *oo = nullptr, *oml = nullptr;
-  if (steps > 0) {
-    const int item = kvh * n_rb + row / rows;
-    const int64_t F = a.n_kv * n_rb * steps, x0 = item * steps;
-    const int w0 = worker_of(x0, F, kPxBlocks);
-    n_pre = worker_of(x0 + steps - 1, F, kPxBlocks) - w0 + 1;
-    po = a.pre_o + ((int64_t)(w0 + item) * rows + row % rows) * HD;
-    pml = a.pre_ml + ((int64_t)(w0 + item) * rows + row % rows) * 2;
-  }
-  if (c1 > c0) {
-    const int item = b * a.n_kv + kvh;
-    const int64_t x0 = c0 * a.n_kv + kvh * (c1 - c0);
-    const int w0 = worker_of(x0, all, kPxListWaves);
-    n_own = worker_of(x0 + (c1 - c0) - 1, all, kPxListWaves) - w0 + 1;
-    oo = a.own_o + ((int64_t)(w0 + item) * 16 + hh) * HD;
-    oml = a.own_ml + ((int64_t)(w0 + item) * 16 + hh) * 2;
-  }
-  const int tid = threadIdx.x, gi = tid / TP, d4 = tid % TP, lane = tid & (kWave - 1), n = n_pre + n_own;
-  auto ml_of = [&](int p) { return p < n_pre ? pml + (int64_t)p * rows * 2 : oml + (int64_t)(p - n_pre) * 32; };
-  auto o_of = [&](int p) {
-    return *reinterpret_cast<const f4_t*>((p < n_pre ? po + (int64_t)p * rows * HD : oo + (int64_t)(p - n_pre) * 16 * HD) + 4 * d4);
-  };
-  float M = -INFINITY, L = 0.f;
-  f4_t O = {0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < n; p0 += kPxMergeThreads) {
-    const int here = min(n - p0, kPxMergeThreads);
-    float m1 = -INFINITY, l1 = 0.f;
-    if (tid < here) {
-      const float* ml = ml_of(p0 + tid);
-      m1 = ml[0];
-      l1 = ml[1];
+  const int hi = cut_len(len, a.max_pages, a.own.shift), t0 = lo >> 5;
+  const int ptiles = (lp + 31) >> 5, mine = hi > lo ? ((hi - 1) >> 5) - t0 + 1 : 0;
+  const bool pre_near = !PIECES || px_prefix_near(a.batch, a.n_kv, ptiles);
+  const int n0 = pre_near ? ptiles : 0, n = n0 + (PIECES ? min(mine, px_near(a)) : mine);
+  const PxKV pre{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
+  const PxKV own{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
+  PxState<HD> st;
+  px_run<HD, F>(st, a, kvh, b * a.g, a.g, wave, n, W, lane, [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) {
+    const bool first = k < n0;
+    px_load<HD, F>(t, first ? pre : own, first ? k : t0 + k - n0, k < n, lane);
+  });
+  if constexpr (PIECES) {
+    const int blocks = (int)a.plan[a.batch + 2];
+    const int64_t steps = a.plan[a.batch + 1];
+    if (steps > 0) {   // the prefix's pieces: the group's rows may lie in two blocks of rows
+      const int row = b * a.g + min(h, a.g - 1), n_rb = (a.batch * a.g + rows - 1) / rows;
+      const int64_t F_ = a.n_kv * n_rb * steps;
+      auto item_of = [&](int r) { return kvh * n_rb + r / rows; };
+      const int i0 = item_of(b * a.g), i1 = item_of(b * a.g + a.g - 1), item = item_of(row);
+      const int w00 = worker_of(i0 * steps, F_, blocks), w01 = worker_of(i0 * steps + steps - 1, F_, blocks);
+      const int w10 = i1 == i0 ? w00 : worker_of(i1 * steps, F_, blocks), w11 = i1 == i0 ? w01 : worker_of(i1 * steps + steps - 1, F_, blocks);
+      const int w0 = item == i0 ? w00 : w10, w1 = item == i0 ? w01 : w11;
+      const float* o = a.pre_o + ((int64_t)(w0 + item) * rows + row % rows) * HD;
+      const float* ml = a.pre_ml + ((int64_t)(w0 + item) * rows + row % rows) * 2;
+#pragma unroll 2
+      for (int p = wave; p <= max(w01 - w00, w11 - w10); p += W)
+        if (w0 + p <= w1) px_absorb<HD>(st, o + (int64_t)p * rows * HD, ml + (int64_t)p * rows * 2, j);
     }
-    f4_t first[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) first[i] = i * G + gi < here ? o_of(p0 + i * G + gi) : f4_t{0.f, 0.f, 0.f, 0.f};
-    const float mw = wave_max(m1);
-    if (p0 > 0) __syncthreads();   // the weights before have been read
-    if (lane == 0) red[0][tid / kWave] = mw;
-    __syncthreads();
-    float Mn = M;
-#pragma unroll
-    for (int w = 0; w < W; ++w) Mn = fmaxf(Mn, red[0][w]);
-    // a row that has seen nothing: m = M = -inf, with l and O of zero
-    const float f = m1 == Mn ? 1.f : __builtin_amdgcn_exp2f(m1 - Mn), f0 = M == Mn ? 1.f : __builtin_amdgcn_exp2f(M - Mn);
-    weight[tid] = f;
-    const float lw = wave_sum(l1 * f);
-    if (lane == 0) red[1][tid / kWave] = lw;
-    __syncthreads();
-    M = Mn;
-    L *= f0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) L += red[1][w];
-    O *= f0;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (i * G + gi < here) O += first[i] * weight[i * G + gi];
-#pragma unroll 4
-    for (int p = kAhead * G + gi; p < here; p += G) O += o_of(p0 + p) * weight[p];
+    const int64_t c0 = a.plan[b], c1 = a.plan[b + 1];
+    if (c1 > c0) {     // the far own tiles' pieces
+      const int item = b * a.n_kv + kvh, workers = (kPxBlocks - blocks) * kPxWaves;
+      const int64_t x0 = c0 * a.n_kv + kvh * (c1 - c0), all = a.plan[a.batch] * a.n_kv;
+      const int w0 = worker_of(x0, all, workers), w1 = worker_of(x0 + (c1 - c0) - 1, all, workers);
+      const float* o = a.own_o + ((int64_t)(w0 + item) * 16 + min(h, a.g - 1)) * HD;
+      const float* ml = a.own_ml + ((int64_t)(w0 + item) * 16 + min(h, a.g - 1)) * 2;
+#pragma unroll 2
+      for (int p = wave; p <= w1 - w0; p += W) px_absorb<HD>(st, o + (int64_t)p * 16 * HD, ml + (int64_t)p * 32, j);
+    }
   }
-  so[gi][d4] = O;
-  __syncthreads();
-  if (gi != 0) return;
+  PxJoin<HD, 1, W> jn;
+  jn.run(st, sm, wave, lane);
+  if (h >= a.g) return;
+  const float inv = jn.L == 0.f ? 0.f : 1.f / jn.L;
+  _Float16* out = a.out + b * a.out_stride + (kvh * a.g + h) * HD + 4 * j;
 #pragma unroll
-  for (int k = 1; k < G; ++k) O += so[k][d4];
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  h4_t v;
+  for (int i = 0; i < jn.PER; ++i) {
+    if (wave + i * W >= DT) continue;
+    h4_t v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (_Float16)(O[i] * inv);
-  *reinterpret_cast<h4_t*>(a.out + b * a.out_stride + head * HD + 4 * d4) = v;
+    for (int e = 0; e < 4; ++e) v[e] = (_Float16)(jn.O[i][e] * inv);
+    *reinterpret_cast<h4_t*>(out + (wave + i * W) * 16) = v;
+  }
 }
 
 // Query rows of a block for R rows per kv head.
@@ -934,7 +1001,7 @@ PxSpace px_space(int batch, int n_heads, int n_kv, int hd) {
   size_t off = 0;
   auto take = [&](size_t n) { const size_t o = off; off += (n + 255) & ~(size_t)255; return o; };
   PxSpace s;
-  s.plan = take((batch + 2) * sizeof(int64_t));
+  s.plan = take((batch + 3) * sizeof(int64_t));
   s.own_ml = take(own * 32 * 4);
   s.own_o = take(own * 16 * hd * 4);
   s.pre_ml = take(pre * 2 * 4);
@@ -951,18 +1018,35 @@ bool px_shape_ok(int batch, int n_heads, int n_kv, int hd) {
 template <int HD, int F, int ROWS>
 void px_launch_rows(const PxArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((px_stage1<HD, F, ROWS>), dim3(kPxBlocks), dim3(kPxThreads), 0, st, a);
-  hipLaunchKernelGGL((px_merge<HD>), dim3(a.batch * a.n_kv * a.g), dim3(kPxMergeThreads), 0, st, a, ROWS, PxForm<HD, F, ROWS>::TPS);
+}
+
+// 8 waves a block while every block has a CU of its own (two sequences of 7B heads over
+// 1000 tokens: 9.4 us, with 4 waves 10.7), then 4, two blocks to a CU (256 over 200: 14.3
+// us, with 8 waves 22.3).
+template <int HD, int F, bool PIECES>
+void px_launch_finish(const PxArgs& a, int rows, hipStream_t st) {
+  const int blocks = a.batch * a.n_kv;
+  if (blocks <= kPxBlocks) hipLaunchKernelGGL((px_finish<HD, F, 8, PIECES>), dim3(blocks), dim3(8 * kWave), 0, st, a, rows);
+  else hipLaunchKernelGGL((px_finish<HD, F, 4, PIECES>), dim3(blocks), dim3(4 * kWave), 0, st, a, rows);
 }
 
 template <int HD, int F>
 void px_launch(const PxArgs& a, hipStream_t st) {
-  switch (px_rows((int64_t)a.batch * a.g)) {
+  // the most that the tables hold: short ones need no first launch
+  const int64_t pre_tiles = (int64_t)a.pre_pages << (a.pre.shift - 5), own_tiles = (int64_t)a.max_pages << (a.own.shift - 5);
+  const int rows = px_rows((int64_t)a.batch * a.g);
+  if (own_tiles <= 64 && px_prefix_near(a.batch, a.n_kv, pre_tiles)) {
+    px_launch_finish<HD, F, false>(a, rows, st);
+    return;
+  }
+  switch (rows) {
     case 16: px_launch_rows<HD, F, 16>(a, st); break;
     case 32: px_launch_rows<HD, F, 32>(a, st); break;
     case 64: px_launch_rows<HD, F, 64>(a, st); break;
     case 128: px_launch_rows<HD, F, 128>(a, st); break;
     default: px_launch_rows<HD, F, 256>(a, st);
   }
+  px_launch_finish<HD, F, true>(a, rows, st);
 }
 
 template <int HD>

@@ -33,9 +33,10 @@ def g():
 
 class Case:
     """A batch of forked sequences (one pool, shared pages first) or, with `apart`, a prefix in a pool of
-    its own and tables that hold only the sequences' own tokens."""
+    its own and tables that hold only the sequences' own tokens.  `pad`: entries of the tables behind those
+    in use (of -1), as a server's tables have: long tables are worked through in two launches, short ones in one."""
 
-    def __init__(self, g, seed, kv, heads, n_kv, hd, page, prefix, own, form="own", apart=False, layers=1, qscale=1.5):
+    def __init__(self, g, seed, kv, heads, n_kv, hd, page, prefix, own, form="own", apart=False, layers=1, qscale=1.5, pad=1):
         rng = self.rng = np.random.default_rng(seed)
         self.g, self.kv, self.heads, self.n_kv, self.hd, self.page, self.prefix = g, kv, heads, n_kv, hd, page, prefix
         self.batch = len(own)
@@ -59,7 +60,8 @@ class Case:
         else:
             self.pre = self.pool
             self.pre_row = shared + ([ids[0]] if n_pre > full else [])
-        self.width = max([len(r) for r in self.rows] + [1]) + 1
+        self.width = max([len(r) for r in self.rows] + [1]) + pad
+        self.pad = pad
         self.q = (rng.standard_normal((self.batch, heads, hd)) * qscale).astype(np.float16)
 
     def want(self):
@@ -98,7 +100,7 @@ class Case:
         for b, r in enumerate(self.rows):
             table[b, :len(r)] = r
         self.host_table = table
-        self.d = dict(q=g.put(q), table=g.put(table), pre=g.i32(self.pre_row + [-1]), plen=g.i32(self.prefix), start=g.i32(self.start),
+        self.d = dict(q=g.put(q), table=g.put(table), pre=g.i32(self.pre_row + [-1] * self.pad), plen=g.i32(self.prefix), start=g.i32(self.start),
                       lens=g.i32(self.lens))
         self.out = g.empty(self.batch * self.os * 2)
         self.ws = g.empty(L.cq_prefix_attention_workspace_bytes(self.batch, self.heads, self.n_kv, self.hd))
@@ -106,7 +108,7 @@ class Case:
 
     def call(self, stream=None, start="start"):
         d = self.d
-        cq.check(L.cq_prefix_attention_decode(d["q"], self.qs, self.out.ptr, self.os, self.pre.arg(), d["pre"], len(self.pre_row) + 1,
+        cq.check(L.cq_prefix_attention_decode(d["q"], self.qs, self.out.ptr, self.os, self.pre.arg(), d["pre"], len(self.pre_row) + self.pad,
                                               d["plen"], self.pool.arg(), d["table"], self.width, d[start] if start else None, d["lens"],
                                               self.batch, self.layer, self.heads, self.ws.ptr, stream))
 
@@ -139,10 +141,28 @@ def test_head_layouts(g, kv, heads, n_kv, hd):
 
 
 @pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("heads,n_kv,hd", SHAPES)
+def test_head_layouts_of_a_long_prefix(g, kv, heads, n_kv, hd):
+    Case(g, heads + 1, kv, heads, n_kv, hd, 64, 2500, [1, 70, 33, 0], layers=2, pad=100).check()
+
+
+@pytest.mark.parametrize("pad", [1, 300])
+@pytest.mark.parametrize("kv", KVS)
 @pytest.mark.parametrize("page", [32, 64, 256])
-@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 64, 255, 256, 257, 1000])
-def test_prefix_lengths(g, kv, page, prefix):
-    Case(g, prefix + page, kv, 6, 2, 64, page, prefix, [0, 1, 31, 32, 65, -1, 300]).check()
+@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 64, 255, 256, 257, 1000, 1792, 1793, 2047, 2048, 2049, 2177, 4000])
+def test_prefix_lengths(g, kv, page, prefix, pad):
+    Case(g, prefix + page, kv, 6, 2, 64, page, prefix, [0, 1, 31, 32, 65, -1, 300], pad=pad).check()
+
+
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("prefix", [0, 40, 2000])
+@pytest.mark.parametrize("batch", [2, 40])
+def test_own_lengths(g, kv, prefix, batch):
+    """Around the own tiles that the second launch takes itself (16 or 64 of them) and past them."""
+    own = [510, 512, 513, 544, 2047, 2048, 2049, 2080, 2500, 5000, 1, 0]
+    own = own[:batch] if batch < 10 else own + [7] * (batch - len(own))
+    Case(g, prefix + batch, kv, 6, 2, 64, 32, prefix, own, pad=40).check()
+    Case(g, prefix + batch, kv, 5, 1, 128, 64, prefix, own[::-1], pad=40, apart=True).check()
 
 
 @pytest.mark.parametrize("kv", KVS)
@@ -160,8 +180,18 @@ def test_batches(g, kv, batch):
     Case(g, batch, kv, 7, 1, 128, 64, 999, rng.integers(0, 60, batch).tolist()).check()
 
 
+@pytest.mark.parametrize("kv", KVS)
+@pytest.mark.parametrize("batch", [1, 2, 3, 5, 9, 10, 16, 19, 33, 37, 64, 74, 130])
+def test_batches_over_a_long_prefix(g, kv, batch):
+    """Every number of rows per block of the first launch, rows that fill the last block or do not."""
+    rng = np.random.default_rng(batch)
+    Case(g, batch, kv, 14, 2, 64, 32, 3333, rng.integers(0, 90, batch).tolist()).check()
+    Case(g, batch, kv, 7, 1, 128, 64, 5000, rng.integers(0, 60, batch).tolist()).check()
+
+
 def test_largest_batch(g):
     rng = np.random.default_rng(1)
+    Case(g, 3, cq.KV_FP8, 3, 1, 64, 64, 700, rng.integers(0, 40, 1024).tolist(), pad=1000).check()
     Case(g, 1, cq.KV_FP16, 2, 1, 64, 32, 100, rng.integers(0, 40, 1024).tolist()).check()
     Case(g, 2, cq.KV_INT8, 2, 2, 64, 32, 2500, rng.integers(0, 40, 1023).tolist()).check()
 
@@ -182,15 +212,17 @@ def test_only_own_tokens_or_nothing(g, kv):
 
 @pytest.mark.parametrize("kv", KVS)
 def test_sharp_and_large_scores(g, kv):
-    """Scores of some tens: the weights of one key or two decide."""
-    Case(g, 11, kv, 14, 2, 64, 64, 500, [20, 100, 3], qscale=12).check()
+    """Scores of some tens: the weights of one key or two decide.  Every form, since each keeps its running maximum."""
+    for batch, prefix in ((3, 500), (2, 2500), (4, 2500), (9, 2500), (18, 2500), (30, 2500)):
+        Case(g, 11, kv, 14, 2, 64, 64, prefix, ([20, 100, 3] * 10)[:batch], qscale=12).check()
 
 
 @pytest.mark.parametrize("kv", [cq.KV_INT8, cq.KV_FP8])
 @pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -20, 2.0 ** 8])
-def test_small_and_large_scales_of_v(g, kv, size):
+@pytest.mark.parametrize("batch,prefix,hd", [(3, 400, 64), (3, 2300, 64), (12, 2300, 128), (40, 2300, 64), (40, 2300, 128)])
+def test_small_and_large_scales_of_v(g, kv, size, batch, prefix, hd):
     """One-byte V whose scales would drive fp16 products into the subnormals, or rows of very different size."""
-    c = Case(g, 12, kv, 7, 1, 64, 32, 400, [50, 3, 77])
+    c = Case(g, 12, kv, 7, 1, hd, 32, prefix, ([50, 3, 77] * 14)[:batch])
     for s in c.pool.scales[1:]:
         s *= np.float32(size) * np.where(c.rng.random(s.shape) < 0.5, 1, 2.0 ** -9).astype(np.float32)
     c.pool.upload()
@@ -202,9 +234,10 @@ def test_small_and_large_scales_of_v(g, kv, size):
 
 @pytest.mark.parametrize("kv", KVS)
 @pytest.mark.parametrize("what", [np.nan, np.inf, -65504.0])
-def test_anything_may_lie_behind_the_lengths(g, kv, what):
+@pytest.mark.parametrize("batch,prefix", [(5, 100), (2, 2500), (5, 2500), (12, 2501), (25, 2497)])
+def test_anything_may_lie_behind_the_lengths(g, kv, what, batch, prefix):
     """Slots past a prefix and past a sequence, before its start, and pages that nobody names."""
-    c = Case(g, 13, kv, 14, 2, 64, 64, 100, [20, 29, 1, 0, 64])
+    c = Case(g, 13, kv, 14, 2, 64, 64, prefix, ([20, 29, 1, 0, 64] * 5)[:batch])
     ref = c.want()
     seen = np.zeros((c.pool.n_pages, c.page), bool)
     for t in range(c.prefix):
@@ -213,7 +246,6 @@ def test_anything_may_lie_behind_the_lengths(g, kv, what):
         for t in range(c.start, n):
             seen[row[t // c.page], t % c.page] = True
     for k in (0, 1):
-        at = c.pool.at[0][~seen.any(-1)]
         for p, t in zip(*np.nonzero(~seen)):
             at = c.pool.at[0, p]
             for h in range(c.n_kv):
@@ -230,10 +262,11 @@ def test_anything_may_lie_behind_the_lengths(g, kv, what):
     assert np.all(np.abs(got[:, :n] - want) <= tol)
 
 
-def test_infinities_and_nan_that_are_seen(g):
+@pytest.mark.parametrize("prefix", [64, 2560])
+def test_infinities_and_nan_that_are_seen(g, prefix):
     """A NaN or an infinite score among the visible keys shows in the rows that see it, and only there."""
-    c = Case(g, 14, cq.KV_FP16, 4, 2, 64, 32, 64, [10, 12, 3])
-    p, t = c.rows[1][2], 3           # an own token of sequence 1, kv head 1
+    c = Case(g, 14, cq.KV_FP16, 4, 2, 64, 32, prefix, [10, 12, 3])
+    p, t = c.rows[1][prefix // 32], 3           # an own token of sequence 1, kv head 1
     c.pool.host[1][c.pool.at[0, p, 1] + c.pool.offsets(1)[t]] = np.nan
     c.pool.upload()
     got = c.run()[:, :c.heads * c.hd].reshape(c.batch, c.heads, c.hd)
@@ -246,11 +279,14 @@ def test_infinities_and_nan_that_are_seen(g):
 
 
 def test_pages_outside_the_pool_are_not_seen(g):
-    for batch in (3, 40):
-        c = Case(g, 15, cq.KV_FP16, 14, 2, 64, 32, 200, [40, 70, 33] + [20] * (batch - 3))
+    for batch, prefix, kv in ((3, 200, cq.KV_FP16), (40, 200, cq.KV_FP8), (2, 2600, cq.KV_INT8), (3, 2600, cq.KV_FP16), (12, 2600, cq.KV_FP8),
+                              (12, 2600, cq.KV_FP16), (40, 2600, cq.KV_FP16), (40, 2600, cq.KV_INT8)):
+        own = ([40, 70, 33] + [20] * batch)[:batch]
+        c = Case(g, 15, kv, 14, 2, 64, 32, prefix, own)
         c.put()
         table = c.host_table.copy()
-        table[1, 7], table[0, 6] = c.pool.n_pages, -2 ** 31     # sequence 1: positions 224..255; sequence 0: 192..223
+        first = prefix // 32                                    # the page of the first own token
+        table[1, first + 1], table[0, first] = c.pool.n_pages, -2 ** 31
         pre = list(c.pre_row)
         pre[2], pre[4] = 2 ** 31 - 1, -1                        # prefix positions 64..95, 128..159
         c.d["table"], c.d["pre"] = g.put(table), g.i32(pre + [-1])
@@ -258,14 +294,14 @@ def test_pages_outside_the_pool_are_not_seen(g):
         c.call()
         got = c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64)[:, :c.heads * c.hd]
         scale, grp = 1 / np.sqrt(c.hd), c.heads // c.n_kv
-        for b in range(3):
+        for b in range(min(3, batch)):
             for h in range(c.heads):
-                K, V = [], []
+                K = []
                 for t in range(c.prefix):
                     if t // 32 not in (2, 4):
                         K.append((c.pre_row[t // 32], t % 32))
                 for t in range(c.prefix, c.lens[b]):
-                    if not (b == 1 and t // 32 == 7) and not (b == 0 and t // 32 == 6):
+                    if not (b == 1 and t // 32 == first + 1) and not (b == 0 and t // 32 == first):
                         K.append((c.rows[b][t // 32], t % 32))
                 pid, tok = (np.array(x) for x in zip(*K))
                 k, v = (c.pool.rows(i, 0, pid)[np.arange(len(pid)), h // grp, tok] for i in (0, 1))
@@ -301,9 +337,10 @@ def test_lengths_are_cut_at_the_tables(g):
     c.check(c.out.to_array(np.float16, (c.batch, c.os)).astype(np.float64))
 
 
-def test_same_bits_on_every_call(g):
+@pytest.mark.parametrize("prefix,batch", [(500, 40), (2900, 3), (2900, 12), (2900, 40)])
+def test_same_bits_on_every_call(g, prefix, batch):
     """Fixed order of all sums: two calls, and a call with a workspace full of NaN, agree bit for bit."""
-    c = Case(g, 18, cq.KV_FP16, 28, 4, 128, 64, 1500, [100, 3, 0, 40, 77] * 8)
+    c = Case(g, 18, cq.KV_FP16, 28, 4, 128, 64, prefix, ([100, 3, 0, 40, 77] * 8)[:batch])
     a = c.run()
     c.ws.upload(np.full(c.ws.nbytes // 2, np.nan, np.float16))
     c.call(start="start")
@@ -313,9 +350,10 @@ def test_same_bits_on_every_call(g):
 
 
 @pytest.mark.parametrize("kv", KVS)
-def test_captured_with_growing_lengths(g, kv):
+@pytest.mark.parametrize("prefix", [300, 2700])
+def test_captured_with_growing_lengths(g, kv, prefix):
     """One graph, replayed as the sequences grow; eager calls of the same state between the replays."""
-    c = Case(g, 19, kv, 14, 2, 64, 64, 300, [200, 40, 90, 33, 64, 1])
+    c = Case(g, 19, kv, 14, 2, 64, 64, prefix, [200, 40, 90, 33, 64, 1], pad=100)
     c.put()
     c.out.upload(np.full((c.batch, c.os), -9, np.float16))
     hip = Hip()
@@ -340,7 +378,7 @@ def test_captured_with_growing_lengths(g, kv):
 def test_two_streams_with_workspaces_of_their_own(g):
     hip = Hip()
     streams = [hip.stream(), hip.stream()]
-    cases = [Case(g, 20 + i, cq.KV_FP16, 14, 2, 64, 32, 500 + i, [9, 70, 3, 40 + i]).put() for i in range(2)]
+    cases = [Case(g, 20 + i, cq.KV_FP16, 14, 2, 64, 32, 2500 + i, [9, 70, 3, 40 + i]).put() for i in range(2)]
     for c in cases:
         c.out.upload(np.full((c.batch, c.os), -9, np.float16))
     cq.synchronize()
