@@ -16,8 +16,8 @@
 //
 // Work of stage 1, whose grid is one block per CU: the steps (a few 32-key tiles) of
 // all items of the prefix, an item being (kv head, block of query rows), form one
-// list that its blocks share evenly, and the far tiles of all (sequence, kv head) items
-// one that the waves of the other blocks share evenly (share_of), wherever item borders
+// list that its blocks share evenly, and the steps of far tiles of all (sequence, kv head) items
+// one that the other blocks share evenly (share_of), wherever item borders
 // fall, from the lengths found on the device: lengths may be ragged, and a captured
 // launch serves other lengths.  Worker w's piece of item i is stored in slot w + i
 // (either w or i grows from one piece to the next, so slots differ), and px_finish
@@ -34,7 +34,6 @@ namespace {
 
 constexpr int kPxWaves = 8, kPxThreads = kPxWaves * kWave;
 constexpr int kPxBlocks = kNumCUs;                    // one block per CU
-constexpr int kPxListWaves = kPxBlocks * kPxWaves;    // most workers of the far own tiles
 constexpr int kPxMaxBatch = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -52,7 +51,9 @@ struct PxArgs {
   int pre_pages, max_pages;
   int batch, n_kv, g;
   // workspace
-  int64_t* plan;                  // [batch + 1] own tiles before each sequence, then the prefix's steps and blocks
+  int64_t* plan;                  // [batch + 1] far own steps before each sequence
+  int* pre_items;                 // first and last worker of each item of the prefix, of each far own item
+  int* own_items;
   float* own_o;                   // [slot][16][HD]
   float* own_ml;                  // [slot][16][2]
   float* pre_o;                   // [slot][rows of a block][HD]
@@ -114,12 +115,12 @@ struct PxKV {
   int lo, hi;
 };
 
-// The K and V of one 32-key tile in matrix operand order, and where its keys are valid.
+// The K and V of one 32-key tile in matrix operand order, and which of its keys are there.
 template <int HD, int F>
 struct PxTile {
   u4_t k[F == CQ_KV_FP16 ? HD / 16 : HD / 32], v[F == CQ_KV_FP16 ? HD / 16 : HD / 32];
   f4_t ks[F == CQ_KV_FP16 ? 1 : 2], vs[F == CQ_KV_FP16 ? 1 : 2];
-  int lo, hi;        // valid keys of the tile: [lo, hi)
+  uint32_t valid;    // a bit per key
 };
 
 // Requests tile ti (positions [32 ti, 32 ti + 32) cut to kv's); with `want` false,
@@ -149,8 +150,8 @@ __device__ __forceinline__ void px_load(PxTile<HD, F>& t, const PxKV& kv, int ti
       t.vs[st] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rvs, (st * 16 + 4 * j) * 4, 0, 0));
     }
   }
-  t.lo = ok ? kv.lo - 32 * ti : 0;
-  t.hi = ok ? kv.hi - 32 * ti : 0;
+  const int lo = max(kv.lo - 32 * ti, 0), hi = min(kv.hi - 32 * ti, 32);
+  t.valid = ok && hi > lo ? (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo) : 0u;
 }
 
 // Operand i of a tile's K (or V) as fp16.
@@ -161,7 +162,7 @@ __device__ __forceinline__ h8_t px_operand(const u4_t* w, int i, uint32_t magic)
 }
 
 // A wave's running softmax over 16 query columns: lane (h, j) holds column h, dims
-// dt * 16 + 4 j + i.  One-byte V: P is rounded to fp16 as p * scale / r, r the power of
+// dt * 16 + 4 j + i, m in log2 units, and in l its own keys' part of the sum.  One-byte V: P is rounded to fp16 as p * scale / r, r the power of
 // two at or below the largest V scale seen (so that small scales do not drive the
 // products into fp16's subnormals), and O is kept in units of r.
 template <int HD>
@@ -186,35 +187,34 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
 #pragma unroll
     for (int a = 0; a < 2; ++a) s[a] *= t.ks[a];
   }
-  const bool part = t.lo > 0 || t.hi < 32;   // wave-uniform
-  if (part) {
+  if (t.valid != 0xffffffffu) {   // wave-uniform
     // masked keys may hold anything, in V too: a weight of 0 does not silence a NaN
-    uint32_t keep[F == CQ_KV_FP16 ? 4 : 2] = {};   // of an operand's 8 keys
+    const uint32_t mine[2] = {t.valid >> (4 * j), t.valid >> (16 + 4 * j)};   // bits of the lane's keys
+    uint32_t in[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int key = (e >> 2) * 16 + 4 * j + (e & 3);
-      const bool in = key >= t.lo && key < t.hi;
-      s[e >> 2][e & 3] = in ? s[e >> 2][e & 3] : -INFINITY;
-      if constexpr (F != CQ_KV_FP16) {
-        t.vs[e >> 2][e & 3] = in ? t.vs[e >> 2][e & 3] : 0.f;
-        keep[e >> 2] |= in ? 0xffu << (8 * (e & 3)) : 0u;
-      } else {
-        keep[e >> 1] |= in ? 0xffffu << (16 * (e & 1)) : 0u;
-      }
+      in[e] = (uint32_t)((int32_t)(mine[e >> 2] << (31 - (e & 3))) >> 31);   // all ones: the key is there
+      const uint32_t x = __float_as_uint(s[e >> 2][e & 3]);
+      s[e >> 2][e & 3] = __uint_as_float((x & in[e]) | (0xff800000u & ~in[e]));
+      if constexpr (F != CQ_KV_FP16) t.vs[e >> 2][e & 3] = __uint_as_float(__float_as_uint(t.vs[e >> 2][e & 3]) & in[e]);
     }
     constexpr int N = sizeof(t.v) / sizeof(t.v[0]);
+    u4_t keep;   // of an operand's 8 keys, or of two operands'
+    if constexpr (F != CQ_KV_FP16) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if constexpr (F != CQ_KV_FP16) t.v[n] &= u4_t{keep[0], keep[1], keep[0], keep[1]};
-      else t.v[n] &= u4_t{keep[0], keep[1], keep[2], keep[3]};
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t lo = __builtin_amdgcn_perm(in[4 * a + 1], in[4 * a], 0x0c0c0400u), hi = __builtin_amdgcn_perm(in[4 * a + 3], in[4 * a + 2], 0x04000c0cu);
+        keep[a] = keep[2 + a] = lo | hi;
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) keep[a] = __builtin_amdgcn_perm(in[2 * a + 1], in[2 * a], 0x05040100u);
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n) t.v[n] &= keep;
   }
-  float mn = st.m;
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mn = fmaxf(mn, s[a][i]);
-  mn = px_col_max(mn);
+  float mn = px_max3(px_max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
+  mn = fmaxf(st.m, px_col_max(px_max3(px_max3(mn, s[1][1], s[1][2]), s[1][3], -INFINITY)) * c2);
   float rn = st.r;
   if constexpr (F != CQ_KV_FP16) {
     float vm = 0.f;
@@ -225,7 +225,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
     rn = fmaxf(rn, __uint_as_float(__float_as_uint(px_col_max(vm)) & 0x7f800000u));
   }
   if (__any(mn > st.m || rn > st.r)) {
-    const float alpha = mn == st.m ? 1.f : __builtin_amdgcn_exp2f((st.m - mn) * c2);
+    const float alpha = mn == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
     const float beta = F != CQ_KV_FP16 ? alpha * (st.r / rn) : alpha;
     st.m = mn;
     st.r = rn;
@@ -233,7 +233,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) st.o[dt] *= beta;
   }
-  const float mm = st.m == -INFINITY ? 0.f : st.m * c2;   // no valid key yet: the masked ones give 0
+  const float mm = st.m == -INFINITY ? 0.f : st.m;   // no valid key yet: the masked ones give 0
   const float ri = F != CQ_KV_FP16 ? 1.f / st.r : 1.f;
   // each weight in two fp16 parts, 22 bits: the matrix units idle here anyway
   h8_t pb, pc;
@@ -255,12 +255,18 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
   }
 }
 
+// Below any V scale that matters (half an fp16 subnormal over 448).
+constexpr float kPxSmallest = 0x1p-40f;
+
 // Tiles ta, ta + step, ... < tb for the rows q[r0 .. r0 + rows) of a kv head: the
-// wave's state, m in log2 units and O in the values' own units.  load(tile, k) requests
-// tile k.
-template <int HD, int F, class Load>
+// wave's state, l complete in every lane and O in the values' own units.  load(tile, k)
+// requests tile k; before() runs while the first tile is on its way.
+// With LONG two copies of the tile's code take turns on two buffers; without, one copy
+// and 64 register moves a tile: code that runs for a tile or two is what an instruction
+// cache filled at 100 cycles a line makes it wait for (a tile's is 2-4 KB).
+template <int HD, int F, bool LONG, class Load, class Before>
 __device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, int kvh, int r0, int rows, int ta, int tb, int step, int lane,
-                                       Load load) {
+                                       Load load, Before before) {
   constexpr int KK = HD / 32, DT = HD / 16;
   const int h = lane & 15, j = lane >> 4;
   const float c2 = kLog2e / sqrtf((float)HD);
@@ -274,39 +280,31 @@ __device__ __forceinline__ void px_run(PxState<HD>& st, const PxArgs& a, int kvh
   for (int kk = 0; kk < KK; ++kk) qb[kk] = __builtin_bit_cast(h8_t, load_u4(q + kk * 32 + j * 8));
   st.m = -INFINITY;
   st.l = 0.f;
-  st.r = 0x1p-100f;
+  st.r = kPxSmallest;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) st.o[dt] = f4_t{0.f, 0.f, 0.f, 0.f};
-  for (int ti = ta; ti < tb; ti += 2 * step) {
-    load(B, ti + step);
-    px_attend<HD, F>(A, qb, st, c2, lane, magic);
-    if (ti + step >= tb) break;
-    load(A, ti + 2 * step);
-    px_attend<HD, F>(B, qb, st, c2, lane, magic);
+  before();
+  if constexpr (LONG) {
+    for (int ti = ta; ti < tb; ti += 2 * step) {
+      load(B, ti + step);
+      px_attend<HD, F>(A, qb, st, c2, lane, magic);
+      if (ti + step >= tb) break;
+      load(A, ti + 2 * step);
+      px_attend<HD, F>(B, qb, st, c2, lane, magic);
+    }
+  } else {
+#pragma unroll 1
+    for (int ti = ta; ti < tb; ti += step) {
+      load(B, ti + step);
+      px_attend<HD, F>(A, qb, st, c2, lane, magic);
+      A = B;
+    }
   }
-  st.m *= c2;
   st.l += __shfl_xor(st.l, 16, kWave);
   st.l += __shfl_xor(st.l, 32, kWave);
   if constexpr (F != CQ_KV_FP16) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) st.o[dt] *= st.r;
-  }
-}
-
-// A piece of the own part: one wave's.
-template <int HD, int F>
-__device__ __forceinline__ void px_own_piece(const PxArgs& a, const PxKV& kv, int kvh, int b, int ta, int tb, float* o, float* ml, int lane) {
-  const int h = lane & 15, j = lane >> 4;
-  PxState<HD> st;
-  px_run<HD, F>(st, a, kvh, b * a.g, a.g, ta, tb, 1, lane,
-                [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) { px_load<HD, F>(t, kv, k, k < tb, lane); });
-  if (h < a.g) {
-#pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) *reinterpret_cast<f4_t*>(o + h * HD + dt * 16 + 4 * j) = st.o[dt];
-    if (j == 0) {
-      ml[2 * h] = st.m;
-      ml[2 * h + 1] = st.l;
-    }
   }
 }
 
@@ -372,24 +370,24 @@ struct PxForm {
   static constexpr int NS = F == CQ_KV_FP16 && 3 * STAGE * 2 <= 96 * 1024 ? 3 : 2;
   static constexpr int DT = HD / 16, CG = WR / 16;
   static constexpr int STATE = 4 + 4 * DT * CG;         // floats of one lane's softmax state in LDS (two slices): (m, l) of each, O
-  // halves of LDS: the stages, over them the states of the other key groups
-  static constexpr int SM = LDS ? std::max(NS * STAGE, (KH - 1) * RG * kWave * STATE * 2) : kPxWaves * 16 * (2 + HD) * 2;
+  // halves of LDS: the states that PxJoin takes; the stages, over them the states of the other key groups
+  static constexpr int SM = std::max({kPxWaves * 16 * (2 + HD) * 2, LDS ? NS * STAGE : 0, LDS ? (KH - 1) * RG * kWave * STATE * 2 : 0});
   static constexpr int SCL = LDS && F != CQ_KV_FP16 ? (NS + 3) * TPS * kTileKeys : 1;   // K scales per slot, V scales three steps
 };
 
-// Tiles [tb, te) of the prefix for up to 64 rows.
-template <int HD, int F, int ROWS>
-__device__ __forceinline__ void px_stream_piece(const PxArgs& a, float* sm, int kvh, int r0, int R, int lp, int tb, int te, float* o,
+// Tiles [tb, te) of a cache for the rows [r0, min(r0 + 16 RG, R)) of a kv head, by the
+// waves of a block in registers.
+template <int HD, int F, int RG>
+__device__ __forceinline__ void px_stream_piece(const PxArgs& a, const PxKV& kv, float* sm, int kvh, int r0, int R, int tb, int te, float* o,
                                                 float* ml) {
-  using P = PxForm<HD, F, ROWS>;
-  constexpr int DT = HD / 16, RG = P::RG, KH = P::KH;
+  constexpr int DT = HD / 16, KH = kPxWaves / RG;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rg = wave % RG, kg = wave / RG, rw = r0 + rg * 16;
-  const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
   PxState<HD> st;
   const int end = rw < R ? te : tb;   // a wave without rows takes no tile
-  px_run<HD, F>(st, a, kvh, min(rw, R - 1), max(min(16, R - rw), 1), tb + kg, end, KH, lane,
-                [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) { px_load<HD, F>(t, kv, k, k < end, lane); });
+  px_run<HD, F, true>(st, a, kvh, min(rw, R - 1), max(min(16, R - rw), 1), tb + kg, end, KH, lane,
+                [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) { px_load<HD, F>(t, kv, k, k < end, lane); },
+                []() {});
   PxJoin<HD, RG, KH> jn;
   jn.run(st, sm, wave, lane);
   const int h = lane & 15, j = lane >> 4;
@@ -811,20 +809,20 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   }
 }
 
-// Blocks that take the prefix, of kPxBlocks; the others take the own part.  Each kind
-// of work has a chain of its own from first load to stored piece (some 7 us), which a
-// block that does both would pay twice.  Costs in block time, microseconds: a step of
-// the prefix, an own tile, an own piece.
+// Blocks that take the prefix, of kPxBlocks; the others take the far own tiles.  Costs
+// in block time, microseconds: a step of the prefix and the chain of a piece of it, an
+// own step.
 template <int HD, int F, int ROWS>
-__device__ __forceinline__ int px_pre_blocks(int64_t pre_steps, int64_t pre_items, int64_t own_tiles, int64_t own_items) {
+__device__ __forceinline__ int px_pre_blocks(int64_t pre_steps, int64_t pre_items, int64_t own_steps) {
   using P = PxForm<HD, F, ROWS>;
-  if (own_tiles == 0) return kPxBlocks;
+  if (own_steps == 0) return kPxBlocks;
   if (pre_steps == 0) return 0;
   constexpr float tile = HD == 128 ? 0.8f : 0.4f;
-  const float pre = (float)pre_steps * (P::TPS * tile * (ROWS <= 64 ? 1.f : ROWS == 128 ? 0.9f : 1.7f)) + (float)min(pre_items, pre_steps) * (P::LDS ? 7.f : 3.f);
-  const float own = (float)own_tiles * (tile * 0.8f) + (float)min(own_items, own_tiles) * 0.4f;
+  const float pre = (float)pre_steps * (P::TPS * tile * (ROWS <= 64 ? 1.f : ROWS == 128 ? 0.9f : 1.7f)) +
+                    (float)min(pre_items, pre_steps) * (P::LDS ? 7.f : 3.f);
+  const float own = (float)own_steps * (kPxWaves * tile);
   int n = (int)((float)kPxBlocks * pre / (pre + own) + 0.5f);
-  n = max(n, kPxBlocks - (int)min((own_tiles + kPxWaves - 1) / kPxWaves, (int64_t)kPxBlocks));   // no more blocks than tiles for their waves
+  n = max(n, kPxBlocks - (int)min(own_steps, (int64_t)kPxBlocks));   // no more blocks than steps
   n = min(n, (int)min(pre_steps, (int64_t)kPxBlocks));
   return min(max(n, 1), kPxBlocks - 1);
 }
@@ -839,13 +837,13 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lp = cut_len((int)load_ctl_u32(a.pre_len), a.pre_pages, a.pre.shift);
   const int lo = a.start ? max((int)load_ctl_u32(a.start), 0) : 0;
-  // far own tiles before each sequence
+  // steps (8 tiles) of far own tiles before each sequence
   const int near = px_near(a);
   int64_t n2[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int b = 2 * threadIdx.x + i, hi = b < a.batch ? cut_len(a.len[b], a.max_pages, a.own.shift) : 0;
-    n2[i] = hi > lo ? max((int64_t)((hi - 1) >> 5) - (lo >> 5) + 1 - near, (int64_t)0) : 0;
+    n2[i] = hi > lo ? (max((int64_t)((hi - 1) >> 5) - (lo >> 5) + 1 - near, (int64_t)0) + kPxWaves - 1) / kPxWaves : 0;
   }
   int64_t x = n2[0] + n2[1];
 #pragma unroll
@@ -861,15 +859,10 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   if (threadIdx.x == 0) cum[0] = 0;
   __syncthreads();
   const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, ptiles = (lp + 31) >> 5, steps = px_prefix_near(a.batch, a.n_kv, ptiles) ? 0 : (ptiles + P::TPS - 1) / P::TPS;
-  const int64_t pre_steps = (int64_t)a.n_kv * n_rb * steps, own_tiles = cum[a.batch] * a.n_kv;
-  const int n_pre = px_pre_blocks<HD, F, ROWS>(pre_steps, a.n_kv * n_rb, own_tiles, (int64_t)a.batch * a.n_kv);
-  if (blockIdx.x == 0) {
+  const int64_t pre_steps = (int64_t)a.n_kv * n_rb * steps, own_steps = cum[a.batch] * a.n_kv;
+  const int n_pre = px_pre_blocks<HD, F, ROWS>(pre_steps, a.n_kv * n_rb, own_steps);
+  if (blockIdx.x == 0)
     for (int b = threadIdx.x; b <= a.batch; b += kPxThreads) a.plan[b] = cum[b];
-    if (threadIdx.x == 0) {
-      a.plan[a.batch + 1] = steps;
-      a.plan[a.batch + 2] = n_pre;
-    }
-  }
   int64_t at, end;
   if ((int)blockIdx.x < n_pre) {
     const int w = blockIdx.x;
@@ -879,14 +872,19 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
       const int sb = (int)min((int64_t)steps, sa + (end - at));
       float *o = a.pre_o + (int64_t)(w + item) * ROWS * HD, *ml = a.pre_ml + (int64_t)(w + item) * ROWS * 2;
       const int tb = sa * P::TPS, te = min(sb * P::TPS, ptiles);
+      if (threadIdx.x == 0 && sa == 0) a.pre_items[2 * item] = w;
+      if (threadIdx.x == 0 && sb == steps) a.pre_items[2 * item + 1] = w;
       if constexpr (P::LDS) px_shared_piece<HD, F, ROWS>(a, smem, scl, kvh, rb * ROWS, R, lp, tb, te, o, ml);
-      else px_stream_piece<HD, F, ROWS>(a, reinterpret_cast<float*>(smem), kvh, rb * ROWS, R, lp, tb, te, o, ml);
+      else {
+        const PxKV kv{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
+        px_stream_piece<HD, F, P::RG>(a, kv, reinterpret_cast<float*>(smem), kvh, rb * ROWS, R, tb, te, o, ml);
+      }
       at += sb - sa;
     }
     return;
   }
-  const int w = (blockIdx.x - n_pre) * kPxWaves + wave;
-  share_of(w, own_tiles, (kPxBlocks - n_pre) * kPxWaves, &at, &end);
+  const int w = blockIdx.x - n_pre;
+  share_of(w, own_steps, kPxBlocks - n_pre, &at, &end);
   while (at < end) {
     int b = 0, top = a.batch;   // last b with n_kv * cum[b] <= at
     while (top - b > 1) {
@@ -894,44 +892,82 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
       if (cum[mid] * a.n_kv <= at) b = mid; else top = mid;
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    const int nt = (int)(cum[b + 1] - cum[b]);
+    const int ns = (int)(cum[b + 1] - cum[b]);
     const int64_t in = at - cum[b] * a.n_kv;
-    const int kvh = (int)px_div(in, nt), ta = (int)(in - (int64_t)kvh * nt), item = b * a.n_kv + kvh;
-    const int tb = (int)min((int64_t)nt, ta + (end - at));
+    const int kvh = (int)px_div(in, ns), sa = (int)(in - (int64_t)kvh * ns), item = b * a.n_kv + kvh;
+    const int sb = (int)min((int64_t)ns, sa + (end - at));
+    if (threadIdx.x == 0 && sa == 0) a.own_items[2 * item] = w;
+    if (threadIdx.x == 0 && sb == ns) a.own_items[2 * item + 1] = w;
     const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = (lo >> 5) + near;
     const PxKV kv{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
-    px_own_piece<HD, F>(a, kv, kvh, b, t0 + ta, t0 + tb, a.own_o + (int64_t)(w + item) * 16 * HD, a.own_ml + (int64_t)(w + item) * 32, lane);
-    at += tb - ta;
+    px_stream_piece<HD, F, 1>(a, kv, reinterpret_cast<float*>(smem), kvh, b * a.g, (b + 1) * a.g, t0 + sa * kPxWaves,
+                              min(t0 + sb * kPxWaves, ((hi - 1) >> 5) + 1), a.own_o + (int64_t)(w + item) * 16 * HD,
+                              a.own_ml + (int64_t)(w + item) * 32);
+    at += sb - sa;
   }
 }
 
-// A piece's state joined into a wave's (whose m is in log2 units, l complete in every
-// lane): o, ml point to the row of this lane.
+// The pieces of one row: row `at` of o and ml is its first, the next lies `stride` rows on.
+struct PxPieces {
+  uint32_t at, stride;
+  int n;
+};
+
+// Running sum of one row's pieces for 4 dims: m, l as in a wave's state.
+struct PxSum {
+  float m, l;
+  f4_t o;
+};
+
+// Pieces p0, p0 + step, ... of a row into s, U requested at a time.
 template <int HD>
-__device__ __forceinline__ void px_absorb(PxState<HD>& st, const float* o, const float* ml, int j) {
-  constexpr int DT = HD / 16;
-  const float m1 = ml[0], l1 = ml[1];
-  f4_t v[DT];
+__device__ __forceinline__ void px_add_pieces(PxSum& s, const float* o, const float* ml, const PxPieces& pc, int p0, int step, int d4) {
+  constexpr int U = 8;
+#pragma unroll 1
+  for (int p = p0; p < pc.n; p += U * step) {
+    float m1[U], l1[U];
+    f4_t v[U];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) v[dt] = *reinterpret_cast<const f4_t*>(o + dt * 16 + 4 * j);
-  const float M = fmaxf(st.m, m1);
-  const float f0 = st.m == M ? 1.f : __builtin_amdgcn_exp2f(st.m - M), f1 = m1 == M ? 1.f : __builtin_amdgcn_exp2f(m1 - M);
-  st.m = M;
-  st.l = st.l * f0 + l1 * f1;
+    for (int u = 0; u < U; ++u) {   // the workspace is smaller than 2^31 bytes
+      const uint32_t at = pc.at + (uint32_t)min(p + u * step, pc.n - 1) * pc.stride;
+      m1[u] = ml[at * 2];
+      l1[u] = ml[at * 2 + 1];
+      v[u] = *reinterpret_cast<const f4_t*>(o + (at * HD + 4 * d4));
+    }
+    float M = s.m;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) st.o[dt] = st.o[dt] * f0 + v[dt] * f1;
+    for (int u = 0; u < U; ++u) {
+      if (p + u * step >= pc.n) m1[u] = -INFINITY;
+      M = fmaxf(M, m1[u]);
+    }
+    const float mm = M == -INFINITY ? 0.f : M;   // nothing seen yet: weights of 0
+    const float f0 = __builtin_amdgcn_exp2f(s.m - mm);
+    s.m = M;
+    s.l *= f0;
+    s.o *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float f = __builtin_amdgcn_exp2f(m1[u] - mm);
+      s.l += l1[u] * f;
+      s.o += v[u] * f;
+    }
+  }
 }
 
-// Block (sequence b, kv head): the near own tiles (and a near prefix's), W waves taking
-// every W-th; then, with PIECES, the pieces that stage 1 left, every W-th too.  The
-// waves join in LDS.
+// Block (sequence b, kv head; rows [per * y, per * (y + 1)) of its group): with PIECES those that stage 1 left, HD / 4 threads to a
+// row and several of its pieces at a time (while the first tiles are on their way);
+// the near own tiles (and a near prefix's), W waves taking every W-th.  All join in LDS.
 template <int HD, int F, int W, bool PIECES>
-__global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int rows) {
+__global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int rows, int per) {
   constexpr int DT = HD / 16;
-  __shared__ __align__(16) float sm[W * 16 * (2 + HD)];
+  constexpr int TP = HD / 4, G = W * kWave / TP;   // threads of a row; rows (or parts of one row's pieces) at a time
+  __shared__ __align__(16) float sm[W * 16 * HD];
+  __shared__ __align__(8) float sml[W * 16 * 2];
+  __shared__ __align__(16) f4_t po_[PIECES ? G : 1][TP];
+  __shared__ float pm_[PIECES ? G : 1], pl_[PIECES ? G : 1];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int h = lane & 15, j = lane >> 4;
-  const int b = blockIdx.x / a.n_kv, kvh = blockIdx.x - b * a.n_kv;
+  const int h = lane & 15;
+  const int rs = blockIdx.y, b = blockIdx.x / a.n_kv, kvh = blockIdx.x - b * a.n_kv;
   const int len = (int)load_ctl_u32(a.len + b);
   const int lp = cut_len((int)load_ctl_u32(a.pre_len), a.pre_pages, a.pre.shift);
   const int lo = a.start ? max((int)load_ctl_u32(a.start), 0) : 0;
@@ -942,51 +978,73 @@ __global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int ro
   const int n0 = pre_near ? ptiles : 0, n = n0 + (PIECES ? min(mine, px_near(a)) : mine);
   const PxKV pre{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
   const PxKV own{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
-  PxState<HD> st;
-  px_run<HD, F>(st, a, kvh, b * a.g, a.g, wave, n, W, lane, [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) {
-    const bool first = k < n0;
-    px_load<HD, F>(t, first ? pre : own, first ? k : t0 + k - n0, k < n, lane);
-  });
+  // rows side by side: a power of two that holds the group's; the other threads share a row's pieces
+  const int row0 = rs * per, own_rows = min(per, a.g - row0);
+  const int rp = per <= 1 ? 1 : 1 << (32 - __builtin_clz(per - 1)), gi = threadIdx.x / TP, d4 = threadIdx.x % TP;
+  const int my = gi & (rp - 1), part = gi / rp, parts = G / rp;
+  PxSum sum{-INFINITY, 0.f, f4_t{0.f, 0.f, 0.f, 0.f}};
+  PxPieces pc[2] = {};
   if constexpr (PIECES) {
-    const int blocks = (int)a.plan[a.batch + 2];
-    const int64_t steps = a.plan[a.batch + 1];
-    if (steps > 0) {   // the prefix's pieces: the group's rows may lie in two blocks of rows
-      const int row = b * a.g + min(h, a.g - 1), n_rb = (a.batch * a.g + rows - 1) / rows;
-      const int64_t F_ = a.n_kv * n_rb * steps;
-      auto item_of = [&](int r) { return kvh * n_rb + r / rows; };
-      const int i0 = item_of(b * a.g), i1 = item_of(b * a.g + a.g - 1), item = item_of(row);
-      const int w00 = worker_of(i0 * steps, F_, blocks), w01 = worker_of(i0 * steps + steps - 1, F_, blocks);
-      const int w10 = i1 == i0 ? w00 : worker_of(i1 * steps, F_, blocks), w11 = i1 == i0 ? w01 : worker_of(i1 * steps + steps - 1, F_, blocks);
-      const int w0 = item == i0 ? w00 : w10, w1 = item == i0 ? w01 : w11;
-      const float* o = a.pre_o + ((int64_t)(w0 + item) * rows + row % rows) * HD;
-      const float* ml = a.pre_ml + ((int64_t)(w0 + item) * rows + row % rows) * 2;
-#pragma unroll 2
-      for (int p = wave; p <= max(w01 - w00, w11 - w10); p += W)
-        if (w0 + p <= w1) px_absorb<HD>(st, o + (int64_t)p * rows * HD, ml + (int64_t)p * rows * 2, j);
-    }
+    // (the lists of pieces are read whether or not there are any: nothing waits for the plan)
+    const int row = b * a.g + row0 + min(my, own_rows - 1), pi = kvh * ((a.batch * a.g + rows - 1) / rows) + row / rows, oi = b * a.n_kv + kvh;
     const int64_t c0 = a.plan[b], c1 = a.plan[b + 1];
-    if (c1 > c0) {     // the far own tiles' pieces
-      const int item = b * a.n_kv + kvh, workers = (kPxBlocks - blocks) * kPxWaves;
-      const int64_t x0 = c0 * a.n_kv + kvh * (c1 - c0), all = a.plan[a.batch] * a.n_kv;
-      const int w0 = worker_of(x0, all, workers), w1 = worker_of(x0 + (c1 - c0) - 1, all, workers);
-      const float* o = a.own_o + ((int64_t)(w0 + item) * 16 + min(h, a.g - 1)) * HD;
-      const float* ml = a.own_ml + ((int64_t)(w0 + item) * 16 + min(h, a.g - 1)) * 2;
-#pragma unroll 2
-      for (int p = wave; p <= w1 - w0; p += W) px_absorb<HD>(st, o + (int64_t)p * 16 * HD, ml + (int64_t)p * 32, j);
-    }
+    const int pw = a.pre_items[2 * pi], pe = a.pre_items[2 * pi + 1], ow = a.own_items[2 * oi], oe = a.own_items[2 * oi + 1];
+    if (!pre_near && my < own_rows) pc[0] = PxPieces{(uint32_t)((pw + pi) * rows + row % rows), (uint32_t)rows, pe - pw + 1};
+    if (c1 > c0 && my < own_rows) pc[1] = PxPieces{(uint32_t)((ow + oi) * 16 + row - b * a.g), 16u, oe - ow + 1};
   }
-  PxJoin<HD, 1, W> jn;
-  jn.run(st, sm, wave, lane);
-  if (h >= a.g) return;
-  const float inv = jn.L == 0.f ? 0.f : 1.f / jn.L;
-  _Float16* out = a.out + b * a.out_stride + (kvh * a.g + h) * HD + 4 * j;
+  PxState<HD> st;
+  px_run<HD, F, false>(
+      st, a, kvh, b * a.g, a.g, wave, n, W, lane,
+      [&](PxTile<HD, F>& t, int k) __attribute__((always_inline)) {
+        const bool first = k < n0;
+        px_load<HD, F>(t, first ? pre : own, first ? k : t0 + k - n0, k < n, lane);
+      },
+      [&]() __attribute__((always_inline)) {
+        if constexpr (PIECES) {
+#pragma unroll 1
+          for (int s = 0; s < 2; ++s)
+            px_add_pieces<HD>(sum, s ? a.own_o : a.pre_o, s ? a.own_ml : a.pre_ml, s ? pc[1] : pc[0], part, parts, d4);
+        }
+      });
+  f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * DT * kWave + lane;
 #pragma unroll
-  for (int i = 0; i < jn.PER; ++i) {
-    if (wave + i * W >= DT) continue;
+  for (int dt = 0; dt < DT; ++dt) w[dt * kWave] = st.o[dt];
+  if (lane < 16) {
+    sml[(wave * 16 + h) * 2] = st.m;
+    sml[(wave * 16 + h) * 2 + 1] = st.l;
+  }
+  if constexpr (PIECES) {
+    po_[gi][d4] = sum.o;
+    if (d4 == 0) pm_[gi] = sum.m, pl_[gi] = sum.l;
+  }
+  __syncthreads();
+  // a thread per (row, 4 dims); rolled loops, for the sake of the instruction cache
+  for (int r = gi; r < own_rows; r += G) {
+    const int row = row0 + r, n_sum = PIECES ? parts : 0;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) M = fmaxf(M, sml[(k * 16 + row) * 2]);
+#pragma unroll 1
+    for (int k = 0; k < n_sum; ++k) M = fmaxf(M, pm_[k * rp + r]);
+    const float mm = M == -INFINITY ? 0.f : M;
+    f4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = 0; k < W; ++k) {
+      const float f = __builtin_amdgcn_exp2f(sml[(k * 16 + row) * 2] - mm);
+      L += sml[(k * 16 + row) * 2 + 1] * f;
+      O += reinterpret_cast<const f4_t*>(sm)[(k * DT + d4 / 4) * kWave + d4 % 4 * 16 + row] * f;
+    }
+#pragma unroll 1
+    for (int k = 0; k < n_sum; ++k) {
+      const float f = __builtin_amdgcn_exp2f(pm_[k * rp + r] - mm);
+      L += pl_[k * rp + r] * f;
+      O += po_[k * rp + r][d4] * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     h4_t v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (_Float16)(jn.O[i][e] * inv);
-    *reinterpret_cast<h4_t*>(out + (wave + i * W) * 16) = v;
+    for (int e = 0; e < 4; ++e) v[e] = (_Float16)(O[e] * inv);
+    *reinterpret_cast<h4_t*>(a.out + b * a.out_stride + (kvh * a.g + row) * HD + 4 * d4) = v;
   }
 }
 
@@ -994,14 +1052,16 @@ __global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int ro
 int px_rows(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
 
 // Workspace: plan, then (m, l) and O of the own pieces and of the prefix's.
-struct PxSpace { size_t plan, own_ml, own_o, pre_ml, pre_o, bytes; };
+struct PxSpace { size_t plan, pre_items, own_items, own_ml, own_o, pre_ml, pre_o, bytes; };
 PxSpace px_space(int batch, int n_heads, int n_kv, int hd) {
   const size_t R = (size_t)batch * (n_heads / n_kv), rows = px_rows(R);
-  const size_t own = kPxListWaves + (size_t)batch * n_kv, pre = (kPxBlocks + n_kv * ((R + rows - 1) / rows)) * rows;
+  const size_t own = kPxBlocks + (size_t)batch * n_kv, pre = (kPxBlocks + n_kv * ((R + rows - 1) / rows)) * rows;
   size_t off = 0;
   auto take = [&](size_t n) { const size_t o = off; off += (n + 255) & ~(size_t)255; return o; };
   PxSpace s;
-  s.plan = take((batch + 3) * sizeof(int64_t));
+  s.plan = take((batch + 1) * sizeof(int64_t));
+  s.pre_items = take(n_kv * ((R + rows - 1) / rows) * 2 * sizeof(int));
+  s.own_items = take((size_t)batch * n_kv * 2 * sizeof(int));
   s.own_ml = take(own * 32 * 4);
   s.own_o = take(own * 16 * hd * 4);
   s.pre_ml = take(pre * 2 * 4);
@@ -1022,12 +1082,16 @@ void px_launch_rows(const PxArgs& a, hipStream_t st) {
 
 // 8 waves a block while every block has a CU of its own (two sequences of 7B heads over
 // 1000 tokens: 9.4 us, with 4 waves 10.7), then 4, two blocks to a CU (256 over 200: 14.3
-// us, with 8 waves 22.3).
+// us, with 8 waves 22.3) unless the group has more rows than 4 waves hold side by side.
+// Where blocks leave CUs idle several take the rows of one group, each with the pieces
+// of its rows (and all of the own tiles).
 template <int HD, int F, bool PIECES>
 void px_launch_finish(const PxArgs& a, int rows, hipStream_t st) {
   const int blocks = a.batch * a.n_kv;
-  if (blocks <= kPxBlocks) hipLaunchKernelGGL((px_finish<HD, F, 8, PIECES>), dim3(blocks), dim3(8 * kWave), 0, st, a, rows);
-  else hipLaunchKernelGGL((px_finish<HD, F, 4, PIECES>), dim3(blocks), dim3(4 * kWave), 0, st, a, rows);
+  const int split = PIECES ? std::max(1, std::min(a.g, kPxBlocks / blocks)) : 1, per = (a.g + split - 1) / split;
+  const dim3 grid(blocks, (a.g + per - 1) / per);
+  if (blocks <= kPxBlocks || a.g > 4 * kWave / (HD / 4)) hipLaunchKernelGGL((px_finish<HD, F, 8, PIECES>), grid, dim3(8 * kWave), 0, st, a, rows, per);
+  else hipLaunchKernelGGL((px_finish<HD, F, 4, PIECES>), grid, dim3(4 * kWave), 0, st, a, rows, per);
 }
 
 template <int HD, int F>
@@ -1097,6 +1161,8 @@ extern "C" int cq_prefix_attention_decode(const void* q, int64_t q_stride, void*
   a.pre_pages = prefix_pages; a.max_pages = max_pages;
   a.batch = batch; a.n_kv = own->n_kv_heads; a.g = n_heads / own->n_kv_heads;
   a.plan = (int64_t*)(ws + s.plan);
+  a.pre_items = (int*)(ws + s.pre_items);
+  a.own_items = (int*)(ws + s.own_items);
   a.own_ml = (float*)(ws + s.own_ml); a.own_o = (float*)(ws + s.own_o);
   a.pre_ml = (float*)(ws + s.pre_ml); a.pre_o = (float*)(ws + s.pre_o);
   const hipStream_t st = (hipStream_t)stream;

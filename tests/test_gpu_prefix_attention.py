@@ -192,6 +192,8 @@ def test_batches_over_a_long_prefix(g, kv, batch):
 def test_largest_batch(g):
     rng = np.random.default_rng(1)
     Case(g, 3, cq.KV_FP8, 3, 1, 64, 64, 700, rng.integers(0, 40, 1024).tolist(), pad=1000).check()
+    for heads, hd in ((16, 128), (9, 128), (16, 64), (8, 128)):
+        Case(g, 4, cq.KV_INT8, heads, 1, hd, 64, 2100, rng.integers(0, 40, 270).tolist(), pad=100).check()
     Case(g, 1, cq.KV_FP16, 2, 1, 64, 32, 100, rng.integers(0, 40, 1024).tolist()).check()
     Case(g, 2, cq.KV_INT8, 2, 2, 64, 32, 2500, rng.integers(0, 40, 1023).tolist()).check()
 
