@@ -6,8 +6,7 @@
 // the sequence's own positions, out = sum exp(s_t - m) v_t / sum exp(s_t - m).  Two
 // launches:
 //   * px_stage1: the prefix, for all rows of a kv head together, in pieces of keys that
-//     leave (m, l, O) in fp32; and of very long sequences the own tiles past the first
-//     few;
+//     leave (m, l, O) in fp32; and the own tiles of very long sequences;
 //   * px_finish: a block per (sequence, kv head) attends over the sequence's own tiles,
 //     joins the pieces of its rows by the log-sum-exp rule and writes the output.
 // Where the tables are short px_finish takes the prefix too, once for each sequence, and
@@ -90,16 +89,24 @@ __device__ __forceinline__ float px_col_max(float v) {
 // One v_max3_f32 (left to the compiler, which knows the wait states of matrix results).
 __device__ __forceinline__ float px_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
-// Own tiles of a sequence that px_finish takes; stage 1 takes those behind them.  With
-// few blocks in the second launch the first one's others are there for them.
-__device__ __forceinline__ int px_near(const PxArgs& a) { return a.batch * a.n_kv <= 64 ? 16 : 64; }
+// Of its n own tiles, how many of a sequence's px_finish takes: all or none; stage 1
+// takes the others, in pieces.  With few blocks in the second launch the first one's
+// are there for sequences of more than a tile per wave (7B heads, 8 sequences over
+// 32640, up to 400 of their own, 13 tiles: 30.5 us both ways; one of 8000: 15.0 us in
+// pieces, 17.8 with the first 16 here; 16 of up to 100: 33.4 here, 38.6 in pieces).
+__device__ __forceinline__ int px_near(const PxArgs& a, int n) {
+  const int most = a.batch * a.n_kv <= 64 ? 8 : 64;
+  return n <= most ? n : 0;
+}
 
-// Whether px_finish takes the prefix: `ptiles` tiles for each of its blocks, against a
-// first launch whose pieces have a chain of their own (some 10 us).  Measured, 7B heads,
-// fp16: 8 sequences over 1500 tokens 11.6 us so and 13.4 in pieces, over 2500 17.4 and
-// 14.5; 64 over 2000 18.0 and 28.5.
-__device__ __host__ __forceinline__ bool px_prefix_near(int batch, int n_kv, int64_t ptiles) {
-  return ptiles * std::max(190, batch * n_kv) <= 190 * 56;
+// Whether px_finish takes the prefix, `ptiles` tiles for each of its `blocks`.  There a
+// tile takes 0.16 us while a block has L2 to itself, blocks * 0.8 ns beyond 190 of them
+// (20 TB/s; one-byte tiles, bound by their conversion, 1.0 ns); in pieces the prefix
+// takes 9 us + 30 ns for each block whose pieces are to be joined.  Measured, here and in
+// pieces, 7B heads, fp16: 8 sequences over 1500 tokens 11.8 and 16.8 us, over 2500 22.5
+// and 16.9; 64 over 3000 26.5 and 28.3; 256 over 800 27.6 and 41, over 1600 44.8 and 43.9.
+__device__ __host__ __forceinline__ bool px_prefix_near(int blocks, int64_t ptiles, bool one_byte) {
+  return ptiles * std::max(190, one_byte ? blocks + blocks / 4 : blocks) <= 11000 + (int64_t)36 * blocks;
 }
 
 // Positions that a table of n pages holds, and the length cut there.
@@ -838,12 +845,12 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   const int lp = cut_len((int)load_ctl_u32(a.pre_len), a.pre_pages, a.pre.shift);
   const int lo = a.start ? max((int)load_ctl_u32(a.start), 0) : 0;
   // steps (8 tiles) of far own tiles before each sequence
-  const int near = px_near(a);
   int64_t n2[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int b = 2 * threadIdx.x + i, hi = b < a.batch ? cut_len(a.len[b], a.max_pages, a.own.shift) : 0;
-    n2[i] = hi > lo ? (max((int64_t)((hi - 1) >> 5) - (lo >> 5) + 1 - near, (int64_t)0) + kPxWaves - 1) / kPxWaves : 0;
+    const int tiles = hi > lo ? ((hi - 1) >> 5) - (lo >> 5) + 1 : 0;
+    n2[i] = (tiles - px_near(a, tiles) + kPxWaves - 1) / kPxWaves;
   }
   int64_t x = n2[0] + n2[1];
 #pragma unroll
@@ -858,7 +865,7 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
   cum[2 * threadIdx.x + 2] = x;
   if (threadIdx.x == 0) cum[0] = 0;
   __syncthreads();
-  const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, ptiles = (lp + 31) >> 5, steps = px_prefix_near(a.batch, a.n_kv, ptiles) ? 0 : (ptiles + P::TPS - 1) / P::TPS;
+  const int R = a.batch * a.g, n_rb = (R + ROWS - 1) / ROWS, ptiles = (lp + 31) >> 5, steps = px_prefix_near(a.batch * a.n_kv, ptiles, F != CQ_KV_FP16) ? 0 : (ptiles + P::TPS - 1) / P::TPS;
   const int64_t pre_steps = (int64_t)a.n_kv * n_rb * steps, own_steps = cum[a.batch] * a.n_kv;
   const int n_pre = px_pre_blocks<HD, F, ROWS>(pre_steps, a.n_kv * n_rb, own_steps);
   if (blockIdx.x == 0)
@@ -898,7 +905,7 @@ __global__ __launch_bounds__(kPxThreads, 2) void px_stage1(const PxArgs a) {
     const int sb = (int)min((int64_t)ns, sa + (end - at));
     if (threadIdx.x == 0 && sa == 0) a.own_items[2 * item] = w;
     if (threadIdx.x == 0 && sb == ns) a.own_items[2 * item + 1] = w;
-    const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = (lo >> 5) + near;
+    const int hi = cut_len((int)load_ctl_u32(a.len + b), a.max_pages, a.own.shift), t0 = lo >> 5;
     const PxKV kv{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
     px_stream_piece<HD, F, 1>(a, kv, reinterpret_cast<float*>(smem), kvh, b * a.g, (b + 1) * a.g, t0 + sa * kPxWaves,
                               min(t0 + sb * kPxWaves, ((hi - 1) >> 5) + 1), a.own_o + (int64_t)(w + item) * 16 * HD,
@@ -974,8 +981,8 @@ __global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int ro
   if (len < 0) return;
   const int hi = cut_len(len, a.max_pages, a.own.shift), t0 = lo >> 5;
   const int ptiles = (lp + 31) >> 5, mine = hi > lo ? ((hi - 1) >> 5) - t0 + 1 : 0;
-  const bool pre_near = !PIECES || px_prefix_near(a.batch, a.n_kv, ptiles);
-  const int n0 = pre_near ? ptiles : 0, n = n0 + (PIECES ? min(mine, px_near(a)) : mine);
+  const bool pre_near = !PIECES || px_prefix_near(a.batch * a.n_kv, ptiles, F != CQ_KV_FP16);
+  const int n0 = pre_near ? ptiles : 0, n = n0 + (PIECES ? px_near(a, mine) : mine);
   const PxKV pre{a.pre, a.pre_layer + kvh * a.pre.head_stride, a.pre_table, 0, lp};
   const PxKV own{a.own, a.own_layer + kvh * a.own.head_stride, a.table + (int64_t)b * a.max_pages, lo, hi};
   // rows side by side: a power of two that holds the group's; the other threads share a row's pieces
@@ -1006,35 +1013,38 @@ __global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int ro
             px_add_pieces<HD>(sum, s ? a.own_o : a.pre_o, s ? a.own_ml : a.pre_ml, s ? pc[1] : pc[0], part, parts, d4);
         }
       });
-  f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * DT * kWave + lane;
+  const int n_w = min(W, n);   // waves that had a tile
+  if (wave < n_w) {
+    f4_t* w = reinterpret_cast<f4_t*>(sm) + wave * DT * kWave + lane;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) w[dt * kWave] = st.o[dt];
-  if (lane < 16) {
-    sml[(wave * 16 + h) * 2] = st.m;
-    sml[(wave * 16 + h) * 2 + 1] = st.l;
+    for (int dt = 0; dt < DT; ++dt) w[dt * kWave] = st.o[dt];
+    if (lane < 16) {
+      sml[(wave * 16 + h) * 2] = st.m;
+      sml[(wave * 16 + h) * 2 + 1] = st.l;
+    }
   }
   if constexpr (PIECES) {
     po_[gi][d4] = sum.o;
     if (d4 == 0) pm_[gi] = sum.m, pl_[gi] = sum.l;
   }
   __syncthreads();
-  // a thread per (row, 4 dims); rolled loops, for the sake of the instruction cache
+  // a thread per (row, 4 dims); loops short in code, for the sake of the instruction cache
   for (int r = gi; r < own_rows; r += G) {
     const int row = row0 + r, n_sum = PIECES ? parts : 0;
     float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) M = fmaxf(M, sml[(k * 16 + row) * 2]);
-#pragma unroll 1
+#pragma unroll 4
+    for (int k = 0; k < n_w; ++k) M = fmaxf(M, sml[(k * 16 + row) * 2]);
+#pragma unroll 4
     for (int k = 0; k < n_sum; ++k) M = fmaxf(M, pm_[k * rp + r]);
     const float mm = M == -INFINITY ? 0.f : M;
     f4_t O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int k = 0; k < W; ++k) {
+#pragma unroll 4
+    for (int k = 0; k < n_w; ++k) {
       const float f = __builtin_amdgcn_exp2f(sml[(k * 16 + row) * 2] - mm);
       L += sml[(k * 16 + row) * 2 + 1] * f;
       O += reinterpret_cast<const f4_t*>(sm)[(k * DT + d4 / 4) * kWave + d4 % 4 * 16 + row] * f;
     }
-#pragma unroll 1
+#pragma unroll 4
     for (int k = 0; k < n_sum; ++k) {
       const float f = __builtin_amdgcn_exp2f(pm_[k * rp + r] - mm);
       L += pl_[k * rp + r] * f;
@@ -1048,13 +1058,18 @@ __global__ __launch_bounds__(W * kWave, 2) void px_finish(const PxArgs a, int ro
   }
 }
 
-// Query rows of a block for R rows per kv head.
-int px_rows(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
+// Query rows of a stage 1 block for R rows per kv head.  Many rows: 128 where a tile is
+// 16 KB (half the pieces' bytes, which is what the end of the launch waits for), else 256
+// (7B heads, 64 sequences over 8160, fp16: 30.0 us with 128, 32.5 with 256; E4M3 over 16000:
+// 54.8 and 48.7; 0.5B heads, 128 over 4000: 25.0 and 20.0).
+int px_rows(int64_t R, int hd, bool one_byte) {
+  return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 || (hd == 128 && !one_byte) ? 128 : 256;
+}
 
 // Workspace: plan, then (m, l) and O of the own pieces and of the prefix's.
 struct PxSpace { size_t plan, pre_items, own_items, own_ml, own_o, pre_ml, pre_o, bytes; };
-PxSpace px_space(int batch, int n_heads, int n_kv, int hd) {
-  const size_t R = (size_t)batch * (n_heads / n_kv), rows = px_rows(R);
+PxSpace px_space(int batch, int n_heads, int n_kv, int hd, bool one_byte) {
+  const size_t R = (size_t)batch * (n_heads / n_kv), rows = px_rows(R, hd, one_byte);
   const size_t own = kPxBlocks + (size_t)batch * n_kv, pre = (kPxBlocks + n_kv * ((R + rows - 1) / rows)) * rows;
   size_t off = 0;
   auto take = [&](size_t n) { const size_t o = off; off += (n + 255) & ~(size_t)255; return o; };
@@ -1098,8 +1113,9 @@ template <int HD, int F>
 void px_launch(const PxArgs& a, hipStream_t st) {
   // the most that the tables hold: short ones need no first launch
   const int64_t pre_tiles = (int64_t)a.pre_pages << (a.pre.shift - 5), own_tiles = (int64_t)a.max_pages << (a.own.shift - 5);
-  const int rows = px_rows((int64_t)a.batch * a.g);
-  if (own_tiles <= 64 && px_prefix_near(a.batch, a.n_kv, pre_tiles)) {
+  constexpr bool ONE = F != CQ_KV_FP16;
+  const int rows = px_rows((int64_t)a.batch * a.g, HD, ONE);
+  if (own_tiles <= 64 && px_prefix_near(a.batch * a.n_kv, pre_tiles, ONE)) {
     px_launch_finish<HD, F, false>(a, rows, st);
     return;
   }
@@ -1108,7 +1124,8 @@ void px_launch(const PxArgs& a, hipStream_t st) {
     case 32: px_launch_rows<HD, F, 32>(a, st); break;
     case 64: px_launch_rows<HD, F, 64>(a, st); break;
     case 128: px_launch_rows<HD, F, 128>(a, st); break;
-    default: px_launch_rows<HD, F, 256>(a, st);
+    default:
+      if constexpr (HD != 128 || ONE) px_launch_rows<HD, F, 256>(a, st);
   }
   px_launch_finish<HD, F, true>(a, rows, st);
 }
@@ -1127,7 +1144,9 @@ void px_format(const PxArgs& a, int fmt, hipStream_t st) {
 using namespace cq;
 
 extern "C" size_t cq_prefix_attention_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim) {
-  return px_shape_ok(batch, n_heads, n_kv_heads, head_dim) ? px_space(batch, n_heads, n_kv_heads, head_dim).bytes : 0;
+  if (!px_shape_ok(batch, n_heads, n_kv_heads, head_dim)) return 0;
+  // of either kind of cache
+  return std::max(px_space(batch, n_heads, n_kv_heads, head_dim, false).bytes, px_space(batch, n_heads, n_kv_heads, head_dim, true).bytes);
 }
 
 extern "C" int cq_prefix_attention_decode(const void* q, int64_t q_stride, void* out, int64_t out_stride,
@@ -1151,7 +1170,7 @@ extern "C" int cq_prefix_attention_decode(const void* q, int64_t q_stride, void*
   if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8 || q_stride > ((int64_t)1 << 40) || out_stride > ((int64_t)1 << 40))
     return fail(CQ_EINVAL, "prefix attention: row strides must be multiples of 8 that hold a row");
   if (prefix_pages < 1 || max_pages < 1) return fail(CQ_EINVAL, "prefix attention: empty tables");
-  const PxSpace s = px_space(batch, n_heads, own->n_kv_heads, own->head_dim);
+  const PxSpace s = px_space(batch, n_heads, own->n_kv_heads, own->head_dim, own->kv_dtype != CQ_KV_FP16);
   char* ws = (char*)workspace;
   PxArgs a{};
   a.q = (const _Float16*)q; a.out = (_Float16*)out; a.q_stride = q_stride; a.out_stride = out_stride;
