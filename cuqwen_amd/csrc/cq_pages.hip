@@ -91,123 +91,95 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(PageView from,
 }
 
 // -------------------------------------------------------------- fork, trim
-// A thread follows one table column through the block's kSeqGroup sequences: rows of
-// siblings name the same page in the same column, so a run of equal pages costs one
-// atomic instead of kSeqGroup (64 forks of a prompt of 313 pages: 2504 atomics instead
-// of 20032).  Integer sums: the order of the atomics does not show.
-constexpr int kSeqGroup = 8, kMapThreads = 512;
+// A block takes kSeqGroup entries, thread (column, entry) with the entry in the lowest
+// lane bits: siblings name the same page in the same column, so the first lane of a run
+// of equal pages counts for the whole run (64 forks of a prompt of 313 pages: 2504 atomics
+// instead of 20032).  Integer sums: the order of the atomics does not show.
+// What bounds them: the launch, three memory round trips (the lists; the lengths; the
+// table) and the fetch of their code, which is why a thread looks after one entry only
+// (a thread following a column through eight entries: fork 7.6 us for 64 x 313, trim 8.8;
+// so 5.4 and 4.8).
+// Lengths are written once every thread of the block has read them; no entry that
+// another block carries out has the same sequence.
+constexpr int kSeqGroup = 8, kMapThreads = 1024, kMapCols = kMapThreads / kSeqGroup;
 
-// CQ_OK, or why sequence ids `mine` of entry i cannot be used: an earlier entry names
-// it (or, with `also`, any entry names `also`).  All threads of the block call it.
+__device__ __forceinline__ int pages_of(int tokens, int page_tokens) { return (int)(((int64_t)tokens + page_tokens - 1) / page_tokens); }
+
+// Whether some k in [0, n) is bad(k) for this thread's entry.  `flags`: a word of LDS.
 template <class Bad>
-__device__ __forceinline__ void find_clashes(int n, int i0, int count, int* flag, Bad bad) {
-  for (int k = threadIdx.x; k < n; k += blockDim.x)
-    for (int q = 0; q < count; ++q)
-      if (bad(k, i0 + q)) flag[q] = 1;
+__device__ __forceinline__ bool entry_clashes(int n, int q, int* flags, Bad bad) {
+  if (threadIdx.x == 0) *flags = 0;
+  bool mine = false;
+#pragma unroll 1
+  for (int k = threadIdx.x / kSeqGroup; k < n; k += kMapCols) mine |= bad(k);
+  __syncthreads();
+  if (mine) atomicOr(flags, 1 << q);
+  __syncthreads();
+  return *flags >> q & 1;
+}
+
+// Adds `sign` to the count of page id (-1: none) for each lane, a run of equal ids among
+// the lanes of one column at once.
+__device__ __forceinline__ void count_pages(int* ref, int n_pages, int id, int q, int sign) {
+  const int left = __shfl_up(id, 1, kWave);   // by every lane, those of entry 0 too
+  const bool same = q > 0 && left == id;
+  const unsigned long long follows = __ballot(same);
+  if (same || id < 0 || id >= n_pages) return;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int run = 1 + __builtin_ctzll(~(follows >> lane >> 1));
+  atomicAdd(ref + id, sign * run);
 }
 
 __global__ __launch_bounds__(kMapThreads) void fork_kernel(cq_page_map m, const int* parent, const int* child, int n,
                                                            int* status) {
-  __shared__ int par[kSeqGroup], chi[kSeqGroup], flag[kSeqGroup], held[kSeqGroup], code[kSeqGroup];
-  const int i0 = blockIdx.x * kSeqGroup, count = min(kSeqGroup, n - i0);
-  if (threadIdx.x < count) {
-    par[threadIdx.x] = parent[i0 + threadIdx.x];
-    chi[threadIdx.x] = child[i0 + threadIdx.x];
-    flag[threadIdx.x] = 0;
-  }
-  __syncthreads();
-  find_clashes(n, i0, count, flag, [&](int k, int i) {
-    const int c = child[k];
-    return c == par[i - i0] || (k < i && c == chi[i - i0]);
+  __shared__ int flags;
+  const int q = threadIdx.x % kSeqGroup, i = blockIdx.x * kSeqGroup + q;
+  const int p = i < n ? parent[i] : -1, c = i < n ? child[i] : -1;
+  const bool ok = p >= 0 && p < m.n_seqs && c >= 0 && c < m.n_seqs;
+  const int len = ok ? m.len[p] : 0, old = ok ? m.len[c] : 0;
+  const bool clash = entry_clashes(n, q, &flags, [&](int k) {
+    const int x = child[k];
+    return x == p || (k < i && x == c);
   });
-  __syncthreads();
-  if (threadIdx.x < count) {
-    const int q = threadIdx.x, p = par[q], c = chi[q];
-    int r = CQ_OK, len = 0;
-    if (p < 0 || p >= m.n_seqs || c < 0 || c >= m.n_seqs) r = CQ_ERANGE;
-    else if (flag[q]) r = CQ_EINVAL;
-    else {
-      len = m.len[p];
-      if (m.len[c] != 0) r = CQ_EINVAL;
-      else if (len < 0 || (int64_t)len > (int64_t)m.max_pages * m.page_tokens) r = CQ_ERANGE;
-      else m.len[c] = len;   // no other entry that is carried out reads or writes this one
-    }
-    code[q] = r;
-    held[q] = r == CQ_OK ? (len + m.page_tokens - 1) / m.page_tokens : 0;
-    status[i0 + q] = r;
+  const int code = !ok ? CQ_ERANGE : clash || old != 0 ? CQ_EINVAL
+                 : len < 0 || (int64_t)len > (int64_t)m.max_pages * m.page_tokens ? CQ_ERANGE : CQ_OK;
+  const int held = code == CQ_OK ? pages_of(len, m.page_tokens) : 0;
+  if (threadIdx.x < kSeqGroup && i < n) {
+    status[i] = code;
+    if (code == CQ_OK) m.len[c] = len;
   }
-  __syncthreads();
-  int widest = 0;
-  for (int q = 0; q < count; ++q) widest = max(widest, held[q]);
-  for (int c = threadIdx.x; c < widest; c += kMapThreads) {
-    int id[kSeqGroup];
-#pragma unroll
-    for (int q = 0; q < kSeqGroup; ++q) id[q] = q < count && c < held[q] ? m.table[(int64_t)par[q] * m.max_pages + c] : -1;
-    int run = -1, times = 0;
-#pragma unroll
-    for (int q = 0; q < kSeqGroup; ++q) {
-      if (q >= count || c >= held[q]) continue;
-      m.table[(int64_t)chi[q] * m.max_pages + c] = id[q];
-      if (id[q] < 0 || id[q] >= m.n_pages) continue;
-      if (id[q] != run) {
-        if (times) atomicAdd(m.ref + run, times);
-        run = id[q]; times = 0;
-      }
-      ++times;
+  for (int col = threadIdx.x / kSeqGroup; __any(col < held); col += kMapCols) {
+    int id = -1;
+    if (col < held) {
+      id = m.table[(int64_t)p * m.max_pages + col];
+      m.table[(int64_t)c * m.max_pages + col] = id;
     }
-    if (times) atomicAdd(m.ref + run, times);
+    count_pages(m.ref, m.n_pages, id, q, 1);
   }
 }
 
 __global__ __launch_bounds__(kMapThreads) void trim_kernel(cq_page_map m, const int* seq, const int* keep, int n, int* status) {
-  __shared__ int sq[kSeqGroup], flag[kSeqGroup], kept[kSeqGroup], held[kSeqGroup];
-  const int i0 = blockIdx.x * kSeqGroup, count = min(kSeqGroup, n - i0);
-  if (threadIdx.x < count) {
-    sq[threadIdx.x] = seq[i0 + threadIdx.x];
-    flag[threadIdx.x] = 0;
+  __shared__ int flags;
+  const int q = threadIdx.x % kSeqGroup, i = blockIdx.x * kSeqGroup + q;
+  const int s = i < n ? seq[i] : -1, want = i < n && keep ? keep[i] : 0;
+  const bool ok = s >= 0 && s < m.n_seqs && want >= 0;
+  const int len = ok ? m.len[s] : 0;
+  const bool clash = entry_clashes(n, q, &flags, [&](int k) { return k < i && seq[k] == s; });
+  const int code = !ok ? CQ_ERANGE : clash ? CQ_EINVAL : len < 0 || (int64_t)len > (int64_t)m.max_pages * m.page_tokens ? CQ_ERANGE : CQ_OK;
+  const bool go = code == CQ_OK && want < len;
+  const int kept = go ? pages_of(want, m.page_tokens) : 0, held = go ? pages_of(len, m.page_tokens) : 0;
+  if (threadIdx.x < kSeqGroup && i < n) {
+    status[i] = code;
+    if (go) m.len[s] = want;
   }
-  __syncthreads();
-  find_clashes(n, i0, count, flag, [&](int k, int i) { return k < i && seq[k] == sq[i - i0]; });
-  __syncthreads();
-  if (threadIdx.x < count) {
-    const int q = threadIdx.x, s = sq[q], want = keep ? keep[i0 + q] : 0;
-    int r = CQ_OK, from = 0, to = 0;
-    if (s < 0 || s >= m.n_seqs || want < 0) r = CQ_ERANGE;
-    else if (flag[q]) r = CQ_EINVAL;
-    else {
-      const int len = m.len[s];
-      if (len < 0 || (int64_t)len > (int64_t)m.max_pages * m.page_tokens) r = CQ_ERANGE;
-      else if (want < len) {
-        from = (want + m.page_tokens - 1) / m.page_tokens;
-        to = (len + m.page_tokens - 1) / m.page_tokens;
-        m.len[s] = want;
-      }
+  for (int col = threadIdx.x / kSeqGroup; __any(col < held); col += kMapCols) {
+    int id = -1;
+    if (col >= kept && col < held) {
+      int* at = m.table + (int64_t)s * m.max_pages + col;
+      id = *at;
+      *at = -1;
     }
-    kept[q] = from;
-    held[q] = to;
-    status[i0 + q] = r;
-  }
-  __syncthreads();
-  int first = 0x7fffffff, last = 0;
-  for (int q = 0; q < count; ++q)
-    if (kept[q] < held[q]) first = min(first, kept[q]), last = max(last, held[q]);
-  for (int64_t c = (int64_t)first + threadIdx.x; c < last; c += kMapThreads) {
-    int id[kSeqGroup];
-#pragma unroll
-    for (int q = 0; q < kSeqGroup; ++q) id[q] = q < count && c >= kept[q] && c < held[q] ? m.table[(int64_t)sq[q] * m.max_pages + c] : -1;
-    int run = -1, times = 0;
-#pragma unroll
-    for (int q = 0; q < kSeqGroup; ++q) {
-      if (q >= count || c < kept[q] || c >= held[q]) continue;
-      m.table[(int64_t)sq[q] * m.max_pages + c] = -1;
-      if (id[q] < 0 || id[q] >= m.n_pages) continue;
-      if (id[q] != run) {
-        if (times) atomicSub(m.ref + run, times);
-        run = id[q]; times = 0;
-      }
-      ++times;
-    }
-    if (times) atomicSub(m.ref + run, times);
+    count_pages(m.ref, m.n_pages, id, q, -1);
   }
 }
 
@@ -223,27 +195,41 @@ inline size_t map_workspace_ints(int n_seqs, int n_pages) {
   return kHead + std::max<size_t>((size_t)5 * n_seqs + n_pages, (size_t)2 * n_pages);
 }
 
-// Exclusive sums over the block; *total: the whole sum.
-template <class T>
-__device__ __forceinline__ T block_scan(T v, T* part, T* total) {
+// Inclusive sum over the wave on DPP lane moves (rows of 16, then across rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);   // row_bcast 15 into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);   // row_bcast 31 into rows 2 and 3
+}
+
+// Exclusive sums of four values over the block at once, and the whole sums.
+struct Four { int v[4]; };
+__device__ __forceinline__ Four block_scan(Four x, Four (*part), Four* total) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  T x = v;
+  Four s;
 #pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const T y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
+  for (int i = 0; i < 4; ++i) s.v[i] = wave_scan(x.v[i]);
+  if (lane == kWave - 1) part[wave] = s;
   __syncthreads();
-  if (lane == kWave - 1) part[wave] = x;
-  __syncthreads();
-  T before = 0, all = 0;
+  Four all = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s.v[i] -= x.v[i];
 #pragma unroll
   for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < wave) before += part[w];
-    all += part[w];
+    const Four p = part[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (w < wave) s.v[i] += p.v[i];
+      all.v[i] += p.v[i];
+    }
   }
   *total = all;
-  return before + x - v;
+  return s;
 }
 
 // Pages [begin, n_pages) in order, kPlanThreads * 4 at a time: calls take(page, rank)
@@ -297,9 +283,10 @@ __device__ __forceinline__ int last_at_most(const int* v, int n, int x) {
 
 __global__ __launch_bounds__(kPlanThreads) void append_plan_kernel(cq_page_map m, const int* add, int n_slots, int* status,
                                                                    int* ws) {
-  __shared__ int part[kPlanWaves], last_of[kMaxSeqs], first_of[kMaxSeqs], flag;
-  __shared__ long long part64[kPlanWaves];
+  __shared__ __align__(16) int last_of[kMaxSeqs];
+  __shared__ int part[kPlanWaves], first_of[kMaxSeqs], flag, near[kMaxSeqs];
   __shared__ int before_of[kMaxSeqs], copy_of[kMaxSeqs];   // pages before; index of the copy, -1: none
+  __shared__ Four part4[kPlanWaves];
   const int s = threadIdx.x, n = m.n_seqs, pt = m.page_tokens;
   int* tok0 = ws + kHead;
   int *len0 = tok0 + n, *csrc = len0 + n, *cdst = csrc + n, *ctok = cdst + n, *list = ctok + n;
@@ -308,39 +295,44 @@ __global__ __launch_bounds__(kPlanThreads) void append_plan_kernel(cq_page_map m
   int a = s < n ? add[s] : 0, len = s < n ? m.len[s] : 0;
   bool bad = a < 0 || len < 0 || len > most || a > most - len;
   if (bad) a = len = 0;
-  const int before = (len + pt - 1) / pt, after = (len + a + pt - 1) / pt;
-  const bool writes = a > 0 && len % pt != 0;   // into the last page it holds
-  int last = -1;
-  if (writes) {
+  const int before = pages_of(len, pt), after = pages_of(len + a, pt);
+  int last = -1, holders = 0;
+  if (a > 0 && len % pt != 0) {   // it writes into the last page it holds
     last = m.table[(int64_t)s * m.max_pages + before - 1];
     if (last < 0 || last >= m.n_pages) bad = true, last = -1;
+    else holders = m.ref[last];
   }
   last_of[s] = last;
   __syncthreads();
   if (bad) flag = 1;
   // writers of this page in earlier sequences: those that leave it for a copy count no longer
   bool copy = false;
-  if (last >= 0) {
+  if (holders > 1) {
     int earlier = 0;
-    for (int q = 0; q < s; ++q) earlier += last_of[q] == last;
-    copy = m.ref[last] - earlier > 1;
+    for (int q = 0; q < s; q += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(last_of + q);
+      earlier += (v.x == last) + (q + 1 < s && v.y == last) + (q + 2 < s && v.z == last) + (q + 3 < s && v.w == last);
+    }
+    copy = holders - earlier > 1;
   }
-  long long tokens;
-  const int t0 = (int)block_scan<long long>(a, part64, &tokens);
-  const bool refused = flag != 0 || tokens > n_slots;   // the scan's barriers lie between
-  int pages, copies;   // at most n_slots / 32 + 2 n_seqs pages
-  const int p0 = block_scan(refused ? 0 : after - before + copy, part, &pages);
-  const int c0 = block_scan(refused ? 0 : (int)copy, part, &copies);
+  // tokens in two halves of 16 bits (their sum may pass 32), pages, copies
+  Four sum;
+  const Four base = block_scan(Four{{a & 0xffff, a >> 16, after - before + copy, copy}}, part4, &sum);
+  const long long tokens = ((long long)sum.v[1] << 16) + sum.v[0];
+  const bool refused = flag != 0 || tokens > n_slots;   // the scan's barrier lies between
+  const int pages = refused ? 0 : sum.v[2], copies = refused ? 0 : sum.v[3];   // pages: at most n_slots / 32 + 2 n_seqs
+  const int t0 = (base.v[1] << 16) + base.v[0], p0 = base.v[2], c0 = base.v[3];
   first_of[s] = p0;
   before_of[s] = before;
   copy_of[s] = copy ? c0 : -1;
   int code = refused ? CQ_ERANGE : CQ_OK;
   if (pages > 0) {
-    const int found = in_page_order(m.ref, 0, m.n_pages, pages, part, [](int, int r) { return r <= 0; },
-                                    [&](int p, int rank) { if (rank < pages) list[rank] = p; });
+    const int found = in_page_order(m.ref, 0, m.n_pages, pages, part, [](int, int r) { return r <= 0; }, [&](int p, int rank) {
+      if (rank < kMaxSeqs) near[rank] = p;
+      else if (rank < pages) list[rank] = p;
+    });
     if (found < pages) code = CQ_ENOMEM;
   }
-  __syncthreads();   // the list is written
   if (s == 0) {
     status[0] = code;
     status[1] = pages;
@@ -360,8 +352,10 @@ __global__ __launch_bounds__(kPlanThreads) void append_plan_kernel(cq_page_map m
     }
     if (a > 0) m.len[s] = len + a;
   }
+  if (pages == 0) return;
+  __syncthreads();   // the list is written
   for (int r = s; r < pages; r += kPlanThreads) {
-    const int p = list[r], q = last_at_most(first_of, n, r);
+    const int p = r < kMaxSeqs ? near[r] : list[r], q = last_at_most(first_of, n, r);
     int col = before_of[q] + r - first_of[q];
     if (copy_of[q] >= 0) {
       --col;   // its own copy of the last page first
