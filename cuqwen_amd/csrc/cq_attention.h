@@ -15,6 +15,25 @@ constexpr int kAttnBlocksTarget = 256;   // one block per CU of MI355X
 constexpr int kMinTilesPerPart = 1;      // short contexts spread over as many blocks as the slots allow
 constexpr int kTileKeys = 32;
 
+// Largest of v over the four lanes that share a column (lane % 16).  The two results
+// of a swap go through variables: a bit cast of an element of the builtin's vector
+// reads its first element whatever the index.
+__device__ __forceinline__ float col_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t x = __float_as_uint(fmaxf(__uint_as_float(a0), __uint_as_float(a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
+}
+
+// One v_max3_f32, and not written as asm: the operands are matrix results, and
+// the compiler adds the wait states that these ask for (and that a register
+// that a product has yet to write asks of its next writer) only in front of
+// instructions of its own.
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
 template <int HD>
 struct KVTile {
   h8_t ka[2][HD / 32];

@@ -57,20 +57,6 @@ struct PaShape {
   static constexpr int SM = std::max({NS * STAGE, (KH - 1) * RG * kWave * STATE * 2, ROWS * OS});
 };
 
-// Largest of v over the four lanes that share a column (lane % 16).
-__device__ __forceinline__ float col_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  v = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
-}
-
-// One v_max3_f32, and not written as asm: the operands are matrix results, and
-// the compiler adds the wait states that these ask for (and that a register
-// that a product has yet to write asks of its next writer) only in front of
-// instructions of its own.
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
-
 template <int HD, int KV8, int KH, int TPW>   // KV8: 0 fp16 cache, CQ_KV_INT8 int8 codes
 __global__ __launch_bounds__(kPaThreads, 2) void pf_attention_kernel(const PfAttnArgs a) {
   using SH = PaShape<HD, KV8, KH, TPW>;

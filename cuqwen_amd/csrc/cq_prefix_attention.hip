@@ -74,21 +74,6 @@ __device__ __forceinline__ void share_of(int w, int64_t F, int W, int64_t* first
 // The worker that has tile x.
 __device__ __forceinline__ int worker_of(int64_t x, int64_t F, int W) { return (int)(F <= W ? x : px_div((x + 1) * W - 1, F)); }
 
-// Largest of v over the four lanes that share a column (lane % 16).  The two results
-// of a swap go through variables: a bit cast of an element of the builtin's vector
-// reads its first element whatever the index.
-__device__ __forceinline__ float px_col_max(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t a0 = a[0], a1 = a[1];
-  const uint32_t x = __float_as_uint(fmaxf(__uint_as_float(a0), __uint_as_float(a1)));
-  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  const uint32_t b0 = b[0], b1 = b[1];
-  return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
-}
-// One v_max3_f32 (left to the compiler, which knows the wait states of matrix results).
-__device__ __forceinline__ float px_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
-
 // Of its n own tiles, how many of a sequence's px_finish takes: all or none; stage 1
 // takes the others, in pieces.  With few blocks in the second launch the first one's
 // are there for sequences of more than a tile per wave (7B heads, 8 sequences over
@@ -220,8 +205,8 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
 #pragma unroll
     for (int n = 0; n < N; ++n) t.v[n] &= keep;
   }
-  float mn = px_max3(px_max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
-  mn = fmaxf(st.m, px_col_max(px_max3(px_max3(mn, s[1][1], s[1][2]), s[1][3], -INFINITY)) * c2);
+  float mn = max3(max3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
+  mn = fmaxf(st.m, col_max(max3(max3(mn, s[1][1], s[1][2]), s[1][3], -INFINITY)) * c2);
   float rn = st.r;
   if constexpr (F != CQ_KV_FP16) {
     float vm = 0.f;
@@ -229,7 +214,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 4; ++i) vm = fmaxf(vm, t.vs[a][i]);
-    rn = fmaxf(rn, __uint_as_float(__float_as_uint(px_col_max(vm)) & 0x7f800000u));
+    rn = fmaxf(rn, __uint_as_float(__float_as_uint(col_max(vm)) & 0x7f800000u));
   }
   if (__any(mn > st.m || rn > st.r)) {
     const float alpha = mn == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
@@ -625,17 +610,17 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
     for (int cg = 0; cg < CG; ++cg) {
       float mx = m[cg];
 #pragma unroll
-      for (int st = 0; st < ST; ++st) mx = px_max3(px_max3(mx, s[st][cg][0], s[st][cg][1]), s[st][cg][2], s[st][cg][3]);
-      mn[cg] = px_col_max(mx);
+      for (int st = 0; st < ST; ++st) mx = max3(max3(mx, s[st][cg][0], s[st][cg][1]), s[st][cg][2], s[st][cg][3]);
+      mn[cg] = col_max(mx);
     }
     if constexpr (KV8) {
       float vm = 0.f;
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const f4_t vs = *reinterpret_cast<const f4_t*>(scl_v + step % 3 * SK + kg * TPW * kTileKeys + st * 16 + 4 * j);
-        vm = px_max3(px_max3(vm, vs[0], vs[1]), vs[2], vs[3]);
+        vm = max3(max3(vm, vs[0], vs[1]), vs[2], vs[3]);
       }
-      rn = fmaxf(r, __uint_as_float(__float_as_uint(px_col_max(vm)) & 0x7f800000u));
+      rn = fmaxf(r, __uint_as_float(__float_as_uint(col_max(vm)) & 0x7f800000u));
     }
   };
   auto rescale = [&]() __attribute__((always_inline)) {   // rare once a row has seen some keys
