@@ -153,6 +153,11 @@ __device__ __forceinline__ h8_t px_operand(const u4_t* w, int i, uint32_t magic)
   else return codes_to_h8<F>(i & 1 ? u2_t{w[i / 2].z, w[i / 2].w} : u2_t{w[i / 2].x, w[i / 2].y}, magic);
 }
 
+// The power of two at or below x >= 0, at most 2^126, and 1 / x for such a power: exact,
+// where a division would be ten instructions.
+__device__ __forceinline__ float px_power(float x) { return fminf(__uint_as_float(__float_as_uint(x) & 0x7f800000u), 0x1p126f); }
+__device__ __forceinline__ float px_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
 // A wave's running softmax over 16 query columns: lane (h, j) holds column h, dims
 // dt * 16 + 4 j + i, m in log2 units, and in l its own keys' part of the sum.  One-byte V: P is rounded to fp16 as p * scale / r, r the power of
 // two at or below the largest V scale seen (so that small scales do not drive the
@@ -213,12 +218,12 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vm = fmaxf(vm, t.vs[a][i]);
-    rn = fmaxf(rn, __uint_as_float(__float_as_uint(col_max(vm)) & 0x7f800000u));
+      for (int i = 0; i < 4; ++i) vm = fmaxf(vm, fabsf(t.vs[a][i]));
+    rn = fmaxf(rn, px_power(col_max(vm)));
   }
   if (__any(mn > st.m || rn > st.r)) {
     const float alpha = mn == st.m ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
-    const float beta = F != CQ_KV_FP16 ? alpha * (st.r / rn) : alpha;
+    const float beta = F != CQ_KV_FP16 ? alpha * (st.r * px_inverse(rn)) : alpha;
     st.m = mn;
     st.r = rn;
     st.l *= alpha;
@@ -226,7 +231,7 @@ __device__ __forceinline__ void px_attend(PxTile<HD, F>& t, const h8_t* qb, PxSt
     for (int dt = 0; dt < DT; ++dt) st.o[dt] *= beta;
   }
   const float mm = st.m == -INFINITY ? 0.f : st.m;   // no valid key yet: the masked ones give 0
-  const float ri = F != CQ_KV_FP16 ? 1.f / st.r : 1.f;
+  const float ri = F != CQ_KV_FP16 ? px_inverse(st.r) : 1.f;
   // each weight in two fp16 parts, 22 bits: the matrix units idle here anyway
   h8_t pb, pc;
 #pragma unroll
@@ -618,9 +623,9 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const f4_t vs = *reinterpret_cast<const f4_t*>(scl_v + step % 3 * SK + kg * TPW * kTileKeys + st * 16 + 4 * j);
-        vm = max3(max3(vm, vs[0], vs[1]), vs[2], vs[3]);
+        vm = max3(max3(vm, fabsf(vs[0]), fabsf(vs[1])), fabsf(vs[2]), fabsf(vs[3]));
       }
-      rn = fmaxf(r, __uint_as_float(__float_as_uint(col_max(vm)) & 0x7f800000u));
+      rn = fmaxf(r, px_power(col_max(vm)));
     }
   };
   auto rescale = [&]() __attribute__((always_inline)) {   // rare once a row has seen some keys
@@ -628,7 +633,7 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) grow |= mn[cg] > m[cg];
     if (__any(grow)) {
-      const float beta = KV8 ? r / rn : 1.f;
+      const float beta = KV8 ? r * px_inverse(rn) : 1.f;
       r = rn;
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
@@ -642,7 +647,7 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   };
   h8_t pb[TPW][CG];
   auto probs = [&](const S_t& s, int step) __attribute__((always_inline)) {   // P^T and the row sums
-    const float ri = KV8 ? 1.f / r : 1.f;
+    const float ri = KV8 ? px_inverse(r) : 1.f;
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
       const float mm = m[cg] == -INFINITY ? 0.f : m[cg] * c2;   // no valid key yet: masked scores give exp2(-inf) = 0

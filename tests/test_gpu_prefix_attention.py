@@ -234,6 +234,21 @@ def test_small_and_large_scales_of_v(g, kv, size, batch, prefix, hd):
     assert np.all(np.abs(got[:, :n] - want) <= tol)
 
 
+@pytest.mark.parametrize("kv", [cq.KV_INT8, cq.KV_FP8])
+@pytest.mark.parametrize("share", [1.0, 0.5])
+@pytest.mark.parametrize("batch,prefix", [(3, 400), (3, 2300), (12, 2300), (40, 2300)])
+def test_scales_below_zero(g, kv, share, batch, prefix):
+    """The store writes no such scale, but the formula takes it, all of them or some."""
+    c = Case(g, 15, kv, 7, 1, 64, 32, prefix, ([50, 3, 77] * 14)[:batch])
+    for s in c.pool.scales:
+        s *= np.where(c.rng.random(s.shape) < share, -1, 1).astype(np.float32)
+    c.pool.upload()
+    got = c.run()
+    n = c.heads * c.hd
+    want, tol = (x.reshape(c.batch, n) for x in c.want())
+    assert np.all(np.abs(got[:, :n] - want) <= tol)
+
+
 @pytest.mark.parametrize("kv", KVS)
 @pytest.mark.parametrize("what", [np.nan, np.inf, -65504.0])
 @pytest.mark.parametrize("batch,prefix", [(5, 100), (2, 2500), (5, 2500), (12, 2501), (25, 2497)])
