@@ -96,7 +96,7 @@ __device__ __host__ __forceinline__ bool px_prefix_near(int blocks, int64_t ptil
 
 // Positions that a table of n pages holds, and the length cut there.
 __device__ __forceinline__ int cut_len(int len, int pages, int shift) {
-  return min(max(len, 0), (int)min((int64_t)pages << shift, (int64_t)0x7fffffff));
+  return min(max(len, 0), pages << shift);   // at most 2^30 (checked by the host)
 }
 
 // Positions [lo, hi) of one kv head of a paged cache.
@@ -1159,7 +1159,9 @@ extern "C" int cq_prefix_attention_decode(const void* q, int64_t q_stride, void*
   const int64_t row = (int64_t)n_heads * own->head_dim;
   if (q_stride < row || out_stride < row || q_stride % 8 || out_stride % 8 || q_stride > ((int64_t)1 << 40) || out_stride > ((int64_t)1 << 40))
     return fail(CQ_EINVAL, "prefix attention: row strides must be multiples of 8 that hold a row");
-  if (prefix_pages < 1 || max_pages < 1) return fail(CQ_EINVAL, "prefix attention: empty tables");
+  constexpr int64_t most = (int64_t)1 << 30;   // tile numbers and their positions stay far below 2^31
+  if (prefix_pages < 1 || max_pages < 1 || (int64_t)prefix_pages * prefix->page_tokens > most || (int64_t)max_pages * own->page_tokens > most)
+    return fail(CQ_EINVAL, "prefix attention: a table holds 1 to 2^30 positions");
   const PxSpace s = px_space(batch, n_heads, own->n_kv_heads, own->head_dim, own->kv_dtype != CQ_KV_FP16);
   char* ws = (char*)workspace;
   PxArgs a{};

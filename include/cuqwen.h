@@ -557,8 +557,8 @@ int cq_paged_kv_load(const cq_kv_pages* pages, int32_t layer, void* k, void* v, 
  * n_kv_heads).  d_start NULL: 0.  Sequences forked from one prompt: `prefix` and `own`
  * are the same pool, d_prefix_table the row of any of them, d_start = d_prefix_len.
  * A row that sees no position is zeros; a row with d_len[b] < 0 is left as it was.
- * Lengths past what a table row holds are cut there; pages outside the pool are not
- * seen.  batch in [0, 1024], up to 16 query heads per kv head; q and out 16-byte
+ * Lengths past what a table row holds (at most 2^30 positions) are cut there; pages
+ * outside the pool are not seen.  batch in [0, 1024], up to 16 query heads per kv head; q and out 16-byte
  * aligned and apart.  `workspace`: cq_prefix_attention_workspace_bytes, 16-byte aligned,
  * of its own for calls that may overlap. */
 int cq_prefix_attention_decode(const void* q, int64_t q_stride, void* out, int64_t out_stride, const cq_kv_pages* prefix,

@@ -441,3 +441,37 @@ def test_prefix_is_a_states_own_cache(g):
             assert np.all(np.abs(got - want) <= tol + slack * np.abs(c.pre.rows(1, 1, [0, 1, 2, 3, 4])).max())
         st.free()
         w.free()
+
+
+@pytest.mark.parametrize("kv", KVS)
+def test_offsets_past_32_bits(g, kv):
+    """Pages whose elements lie past 2^32 of the pool's first: every step gives the bits that it gives in a small pool."""
+    heads, n_kv, hd, page, prefix, own = 6, 2, 64, 32768, 3000, 70
+    rng = np.random.default_rng(16)
+    n = prefix + 2 * own
+    rows = [(rng.standard_normal((n, n_kv * hd))).astype(np.float16) for _ in range(2)]
+    q = g.put((rng.standard_normal((2, heads * hd)) * 1.5).astype(np.float16))
+    got = []
+    for ids, n_pages in (((0, 1, 2, 3), 4), ((1040, 1099, 3, 1057), 1100)):
+        d = cq.kv_pages(page, n_kv, hd, n_pages, 1, kv)
+        size, scales = cq.kv_pages_bytes(d)
+        d.k, d.v = (g.empty(size).value for _ in range(2))
+        if scales:
+            d.k_scale, d.v_scale = (g.empty(scales).value for _ in range(2))
+        pool = ctypes.byref(d)
+        slots = [ids[0] * page + t for t in range(prefix)] + [i * page + t for i in ids[1:3] for t in range(own)]
+        cq.check(L.cq_paged_kv_store(pool, 0, g.put(rows[0]), g.put(rows[1]), n_kv * hd, g.i32(slots), n, None))
+        status = g.empty(4)
+        cq.check(L.cq_pages_copy(pool, pool, g.i32([ids[1]]), g.i32([ids[3]]), 1, status.ptr, None))   # the first one's own page
+        assert status.to_array(np.int32, (1,))[0] == 0
+        out, ws = g.empty(2 * heads * hd * 2), g.empty(L.cq_prefix_attention_workspace_bytes(2, heads, n_kv, hd))
+        cq.check(L.cq_prefix_attention_decode(q, heads * hd, out.ptr, heads * hd, pool, g.i32([ids[0]]), 1, g.i32([prefix]), pool,
+                                              g.i32([ids[3], ids[2]]), 1, None, g.i32([own, own]), 2, 0, heads, ws.ptr, None))
+        back = [g.empty(n * n_kv * hd * 2) for _ in range(2)]
+        cq.check(L.cq_paged_kv_load(pool, 0, back[0].ptr, back[1].ptr, n_kv * hd, g.i32(slots), n, None))
+        got.append([x.to_array(np.uint16, (x_n,)) for x, x_n in ((out, 2 * heads * hd), (back[0], n * n_kv * hd), (back[1], n * n_kv * hd))])
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+    if kv == cq.KV_FP16:
+        assert np.array_equal(got[0][1], rows[0].view(np.uint16).ravel()) and np.array_equal(got[0][2], rows[1].view(np.uint16).ravel())
+    assert np.any(got[0][0])

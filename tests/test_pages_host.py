@@ -144,6 +144,9 @@ def test_arguments_of_the_attention():
                 dict(pp=-1), dict(batch=-1), dict(batch=1025), dict(layer=-1), dict(layer=2), dict(heads=0), dict(heads=3),
                 dict(heads=34), dict(own=_pool(kv=1)), dict(own=_pool(n_kv=1)), dict(own=_pool(hd=128)), dict(pre=_pool(layers=1), layer=1)):
         refused(call(**bad))
+    # a table's row of more than 2^30 positions (the pool's pages have 64)
+    for bad in (dict(pp=(1 << 24) + 1), dict(mp=(1 << 24) + 1), dict(pp=(1 << 31) - 1), dict(mp=(1 << 31) - 1)):
+        refused(call(**bad))
     cq.check(call(batch=0, q=None, out=None))
 
 
