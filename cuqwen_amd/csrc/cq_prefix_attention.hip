@@ -398,6 +398,21 @@ __device__ __forceinline__ void px_stream_piece(const PxArgs& a, const PxKV& kv,
   }
 }
 
+// Asks the compiler for N groups of MF matrix and VA vector instructions with the LDS reads
+// of their operands AHEAD groups before them; left to itself it reads each operand where
+// it is used.  (7B heads, 64 sequences over 65280, fp16: 105.6 -> 102.6 us; one-byte
+// tiles, with their scales to read, 70.0 -> 71.7 over 32640, so not there.)
+template <int ID, int AHEAD, int N, int MF, int VA>
+__device__ __forceinline__ void px_interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, ID);   // LDS reads
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    __builtin_amdgcn_sched_group_barrier(0x8, MF, ID);
+    __builtin_amdgcn_sched_group_barrier(0x2, VA, ID);
+    if (q < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 1, ID);
+  }
+}
+
 // Tiles [tb, te) of the prefix for 128 or 256 rows: the prefill attention's loop
 // over pages, without its causal limits.
 template <int HD, int F, int ROWS>
@@ -416,41 +431,49 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   const float c2 = kLog2e / sqrtf((float)HD);
   const int64_t head = a.pre_layer + kvh * a.pre.head_stride;
 
-  // Pages of a step's tiles, one step ahead of the requests that need them; tiles past
-  // the range repeat its last one (and are masked).  A page outside the pool is read
-  // as page 0 and its keys masked: `bad` holds TPS bits per step, the latest lowest.
-  struct Ids { int page[TPS]; };
+  // Where the tiles lie: lane i holds the byte offset of tile i of the next 64, from a
+  // vector's worth of table entries, and a step takes its own with lane reads (as scalar
+  // code, two 64-bit products and sums per tile and step, this was a third of the loop's
+  // instructions).  Tiles past the range repeat its last one (and are masked).  A page
+  // outside the pool is read as page 0 and its keys masked: `bad` holds TPS bits per
+  // step, the latest lowest.
+  struct Tiles { int64_t off[TPS]; };
+  static_assert(kWave % TPS == 0, "whole steps per look-up");
+  constexpr uint32_t BITS = (1u << TPS) - 1;
+  int64_t lane_off = 0;
+  unsigned long long lane_bad = 0;
   uint32_t bad = 0;
   auto tile_at = [&](int ti) __attribute__((always_inline)) { return min(ti, te - 1); };
-  auto fetch = [&](int step) __attribute__((always_inline)) {
-    Ids r;
-    uint32_t b = 0;
+  auto look_up = [&](int step) __attribute__((always_inline)) {   // called for every step in turn
+    constexpr int PER = kWave / TPS;
+    const int first = step % PER * TPS;
+    if (first == 0) {
+      const int ti = tile_at(tb + step * TPS + lane), page = a.pre_table[ti >> s5];
+      const bool ok = page >= 0 && page < a.pre.n_pages;
+      lane_off = (head + (int64_t)(ok ? page : 0) * a.pre.page_stride + (int64_t)(ti & ((1 << s5) - 1)) * TILE) * ES;
+      lane_bad = __ballot(!ok);
+    }
+    Tiles r;
 #pragma unroll
     for (int i = 0; i < TPS; ++i) {
-      const int p = (int)load_ctl_u32(a.pre_table + (tile_at(tb + step * TPS + i) >> s5));
-      const bool ok = p >= 0 && p < a.pre.n_pages;
-      r.page[i] = ok ? p : 0;
-      b |= ok ? 0u : 1u << i;
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)lane_off, first + i), hi = __builtin_amdgcn_readlane((int)(lane_off >> 32), first + i);
+      r.off[i] = (int64_t)((uint64_t)hi << 32 | lo);
     }
-    bad = (bad << TPS) | b;
+    bad = (bad << TPS) | ((uint32_t)(lane_bad >> first) & BITS);
     return r;
-  };
-  // element offset of tile `i` of a step whose pages are `id`
-  auto tile_off = [&](const Ids& id, int step, int i) __attribute__((always_inline)) {
-    return head + (int64_t)id.page[i] * a.pre.page_stride + (int64_t)(tile_at(tb + step * TPS + i) & ((1 << s5) - 1)) * TILE;
   };
   // fp16 cache: straight into LDS, 1 KB per wave instruction, no registers
   constexpr int TB = TILE * 2 / 1024, PW = TPS * TB / kPxWaves;   // KB of a tile's K (or V); instructions per wave and step
   static_assert(KV8 || PW * kPxWaves == TPS * TB, "whole pieces per wave");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-  const uint32_t lane16 = lane * 16;
-  auto dma = [&](const Ids& id, int step, int part) __attribute__((always_inline)) {
+  const uint32_t in_tile = (wave % TB * kWave + lane) * 16;   // of the wave's pieces
+  auto dma = [&](const Tiles& tl, int step, int part) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       const int p = i * kPxWaves + wave;
       // tile of the piece: i (8 KB tiles) or 2 i and 2 i + 1 (4 KB tiles)
-      const int64_t off = TB == 8 ? tile_off(id, step, i) : wave < 4 ? tile_off(id, step, i * 2 % TPS) : tile_off(id, step, (i * 2 + 1) % TPS);
-      lds_load_1k(lds0 + ((step % NS) * P::STAGE + part * TPS * TILE) * 2 + p * 1024, lane16, a.pre.kv[part] + off * 2 + p % TB * 1024);
+      const int64_t off = TB == 8 ? tl.off[i] : wave < 4 ? tl.off[i * 2 % TPS] : tl.off[(i * 2 + 1) % TPS];
+      lds_load_1k(lds0 + ((step % NS) * P::STAGE + part * TPS * TILE) * 2 + p * 1024, in_tile, a.pre.kv[part] + off);
     }
   };
   // keys that are not there may hold anything: keep them out of P*V (each wave clears
@@ -478,14 +501,14 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   struct Pieces { u4_t w[QL]; float s[2]; };
   constexpr int SK = TPS * kTileKeys;
   float *scl_k = scl, *scl_v = scl + NS * SK;   // V scales come with the K of their step, so three slots
-  auto load = [&](Pieces& r, const Ids& id, int step, int part, uint32_t bits) __attribute__((always_inline)) {
+  auto load = [&](Pieces& r, const Tiles& tl, int step, int part, uint32_t bits) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
       const int c = FULL ? i * kPxThreads + threadIdx.x : min((int)threadIdx.x, TPS * TP - 1);
       int64_t off = 0;
 #pragma unroll
       for (int n = 0; n < TPS; ++n)
-        if (c / TP == n) off = tile_off(id, step, n);
+        if (c / TP == n) off = tl.off[n];
       r.w[i] = load_u4(a.pre.kv[part] + off + c % TP * 16);
     }
     if (part == 0 && threadIdx.x < SK) {
@@ -493,7 +516,7 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
       int64_t off = 0;
 #pragma unroll
       for (int i = 0; i < TPS; ++i)
-        if (n == i) off = tile_off(id, step, i);
+        if (n == i) off = tl.off[i];
       off = off / HD + c % kTileKeys;
       const bool in = key < lim && !(bits >> n & 1) && tb + step * TPS + n < te;
       r.s[0] = in ? a.pre.scale[0][off] : 0.f;
@@ -526,29 +549,27 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   };
   // Group g = (K of step g + 1, V of step g), requested NS - 1 steps ahead.
   Pieces pk, pv8;
-  Ids id_v = fetch(0), id_k = id_v, id_n;
-  constexpr uint32_t BITS = (1u << TPS) - 1;
+  Tiles tv = look_up(0);   // of the V to be requested next
   auto request = [&](int g) __attribute__((always_inline)) {
+    const Tiles tk = look_up(g + 1);
     if constexpr (KV8) {
-      load(pk, id_k, g + 1, 0, bad >> TPS & BITS);
-      load(pv8, id_v, g, 1, 0);
+      load(pk, tk, g + 1, 0, bad & BITS);
+      load(pv8, tv, g, 1, 0);
     } else {
-      dma(id_k, g + 1, 0);
-      dma(id_v, g, 1);
+      dma(tk, g + 1, 0);
+      dma(tv, g, 1);
     }
-    id_v = id_k;
-    id_k = id_n;
-    id_n = fetch(g + 3);
+    tv = tk;
   };
-  // Group g in LDS for every wave (its readers' slots free since the last barrier).  The
-  // pages of step g + NS + 1 have been fetched by then.
+  // Group g in LDS for every wave (its readers' slots free since the last barrier).
+  // Step g + NS - 1 has been looked up last by then.
   auto arrive = [&](int g) __attribute__((always_inline)) {
     if constexpr (KV8) {
       store(pk, g + 1, 0, 0);
-      store(pv8, g, 1, bad >> (NS + 1) * TPS & BITS);
+      store(pv8, g, 1, bad >> (NS - 1) * TPS & BITS);
     } else {
       wait_vm<(NS - 2) * 2 * PW>();
-      clear_tail(g, bad >> (NS + 1) * TPS & BITS);
+      clear_tail(g, bad >> (NS - 1) * TPS & BITS);
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
     lds_barrier();
@@ -683,15 +704,13 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
   S_t sa, sb;
   __syncthreads();   // the piece before has left LDS
   const uint32_t bad0 = bad & BITS;
-  id_k = fetch(1);
-  id_n = fetch(2);
   if constexpr (KV8) {
-    load(pk, id_v, 0, 0, bad0);
+    load(pk, tv, 0, 0, bad0);
     store(pk, 0, 0, 0);
     request(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);
   } else {
-    dma(id_v, 0, 0);
+    dma(tv, 0, 0);
 #pragma unroll
     for (int g = 0; g < NS - 1; ++g) request(g);
     wait_vm<(NS - 1) * 2 * PW>();
@@ -709,15 +728,17 @@ __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem,
     __builtin_amdgcn_sched_barrier(0);
     qk(nxt, n + 1);
     probs(cur, n);
+    if constexpr (!KV8) px_interleave<0, 4, ST * KK, CG, 8>();
     // P(n) is formed here, among the matrix instructions of S(n + 1), not moved down to its use
 #pragma unroll
     for (int tw = 0; tw < TPW; ++tw)
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) asm volatile("" : "+v"(pb[tw][cg]));
     __builtin_amdgcn_sched_barrier(0);
-    scale_mask(nxt, n + 1, bad >> (NS + 1) * TPS & BITS);   // fetched: up to step n + NS + 2
+    scale_mask(nxt, n + 1, bad >> (NS - 1) * TPS & BITS);   // looked up: up to step n + NS
     pv(n);
     row_max(nxt, n + 1);
+    if constexpr (!KV8) px_interleave<1, 8, TPW * DT, CG, 4>();
     rescale();
     arrive(n + 1);
   };
