@@ -13,6 +13,15 @@
 // is the only launch; where only the lengths are short (known on the device alone) it
 // does so behind a first launch with nothing to do.
 //
+// What bounds it (per kernel, 7B heads, fp16 unless said otherwise):
+//   * two answers to a short question: the launch (0.5B heads, 100 tokens: one of 4.0 us);
+//   * up to 16 rows a kv head: HBM (2 sequences: 13.7 us for each further 32640 tokens,
+//     4.9 TB/s; a plain copy 4.9), behind about 16 us of two launches, their code, which
+//     comes cold from L2 in 64-byte lines, and the joining;
+//   * 64 sequences (448 rows): waves that wait for each other (px_shared_piece);
+//   * own tokens: HBM (64 sequences with up to 1000: px_finish reads 89 MB, pieces
+//     included, in 22.8 us, 3.9 TB/s).
+//
 // Work of stage 1, whose grid is one block per CU: the steps (a few 32-key tiles) of
 // all items of the prefix, an item being (kv head, block of query rows), form one
 // list that its blocks share evenly, and the steps of far tiles of all (sequence, kv head) items
@@ -159,9 +168,10 @@ __device__ __forceinline__ float px_power(float x) { return fminf(__uint_as_floa
 __device__ __forceinline__ float px_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 
 // A wave's running softmax over 16 query columns: lane (h, j) holds column h, dims
-// dt * 16 + 4 j + i, m in log2 units, and in l its own keys' part of the sum.  One-byte V: P is rounded to fp16 as p * scale / r, r the power of
-// two at or below the largest V scale seen (so that small scales do not drive the
-// products into fp16's subnormals), and O is kept in units of r.
+// dt * 16 + 4 j + i, m in log2 units, and in l its own keys' part of the sum.  One-byte V:
+// P is rounded to fp16 as p * scale / r, r the power of two at or below the largest V
+// scale seen (so that small scales do not drive the products into fp16's subnormals), and
+// O is kept in units of r.
 template <int HD>
 struct PxState {
   float m, l, r;
@@ -373,7 +383,10 @@ struct PxForm {
 };
 
 // Tiles [tb, te) of a cache for the rows [r0, min(r0 + 16 RG, R)) of a kv head, by the
-// waves of a block in registers.
+// waves of a block in registers.  Up to 32 rows HBM bounds it (0.34 us a 32-key E4M3 tile
+// and CU, HD 128); 33 to 64 rows over one-byte tiles their conversion, which each of up to
+// four row groups does for itself (0.72 us).  Two slices of rows a wave, converted once,
+// spill 40 registers and take 44.4 us where this takes 38.4 (8 sequences over 65280, E4M3).
 template <int HD, int F, int RG>
 __device__ __forceinline__ void px_stream_piece(const PxArgs& a, const PxKV& kv, float* sm, int kvh, int r0, int R, int tb, int te, float* o,
                                                 float* ml) {
@@ -414,7 +427,14 @@ __device__ __forceinline__ void px_interleave() {
 }
 
 // Tiles [tb, te) of the prefix for 128 or 256 rows: the prefill attention's loop
-// over pages, without its causal limits.
+// over pages, without its causal limits.  64 sequences of 7B heads, fp16: 41 us for each
+// further 32640 tokens, 730 TFLOP/s.  Over the launch at 32640 tokens the matrix units are
+// busy for 21 % of the cycles, LDS for 12 %, and waves wait for 45 %: of the 46 us that the
+// loop took before its addresses came from lanes, 14 went with the requests taken out, 9
+// with the LDS reads, 8 with most of the PV products, 5 with the exponentials.  Tried and no
+// faster: a tile a wave and step with three or four slots (47 us), V requested and awaited
+// at the middle of a step (41), a wave priority by key group (41), one copy of the step in
+// the code (48), the next operand's reads fully ahead (42).
 template <int HD, int F, int ROWS>
 __device__ __forceinline__ void px_shared_piece(const PxArgs& a, _Float16* smem, float* scl, int kvh, int r0, int R, int lp, int tb, int te,
                                                 float* o_out, float* ml_out) {
