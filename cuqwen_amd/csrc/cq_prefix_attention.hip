@@ -87,7 +87,9 @@ __device__ __forceinline__ int worker_of(int64_t x, int64_t F, int W) { return (
 // takes the others, in pieces.  With few blocks in the second launch the first one's
 // are there for sequences of more than a tile per wave (7B heads, 8 sequences over
 // 32640, up to 400 of their own, 13 tiles: 30.5 us both ways; one of 8000: 15.0 us in
-// pieces, 17.8 with the first 16 here; 16 of up to 100: 33.4 here, 38.6 in pieces).
+// pieces, 17.8 with the first 16 here; 16 of up to 100: 33.4 here, 38.6 in pieces; 16 of up
+// to 1500: 45.8 with up to 16 here, 40.2 in pieces; 14B heads, E4M3, 8 over 20001, of up to
+// 300: 29.4 and 32.3).
 __device__ __forceinline__ int px_near(const PxArgs& a, int n) {
   const int most = a.batch * a.n_kv <= 64 ? 8 : 64;
   return n <= most ? n : 0;
