@@ -485,7 +485,8 @@ typedef struct cq_page_map {
 /* The calls below are asynchronous on `stream`, allocate nothing and take their
  * lists from device memory, so they can be captured; what they find wrong there
  * they report in d_status (device memory, CQ_* codes) and leave alone.  Calls on
- * one map or pool belong on one stream, or in an order of the caller's. */
+ * one map or pool belong on one stream, or in an order of the caller's; a workspace
+ * serves one call at a time, captured ones too. */
 
 /* Each sequence d_child[i] (empty: len 0) becomes a copy of d_parent[i]: the same
  * pages, counted once more; n is at most 1024.  d_status[i] (n ints): CQ_OK; CQ_ERANGE: an id outside
